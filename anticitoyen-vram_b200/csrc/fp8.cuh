@@ -1,0 +1,118 @@
+// e4m3 values with a float scale for each group of 128 (of a row) or block of 128 x 128 (of a weight).
+//
+//   a = max |x| over the group,  s = max(a / 448, 2^-126),  r = 1 / s,  q = e4m3(x r)        (448: the largest e4m3 number)
+//
+// Every step is a correctly rounded float operation, so q and s depend on the group's values alone.  The floor of 2^-126 keeps s
+// a normal number, r finite and a group of zeros at q = 0.  A group that holds a NaN has s = NaN and every q NaN; one that holds an
+// infinity has s = inf, its finite values become 0 and the infinity NaN: whatever product reads the row then gives NaN.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+#define FP8_GROUP 128
+
+struct Fp8Scale { float s, r; };
+
+// `amax`: the bits of the group's largest magnitude; magnitudes are ordered as their bits are, NaNs above infinity
+__device__ __forceinline__ Fp8Scale fp8_scale(uint32_t amax) {
+    float s = __fdiv_rn(__uint_as_float(amax), 448.f);
+    if (s < 1.17549435e-38f) s = 1.17549435e-38f;
+    return {s, __frcp_rn(s)};
+}
+__device__ __forceinline__ uint32_t fp8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// four values times r as e4m3, the first in the lowest byte (beyond 448 by the rounding of r alone: that is 448; NaN stays NaN)
+__device__ __forceinline__ uint32_t fp8_pack4(float a, float b, float c, float d, float r) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * r, b * r), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * r, d * r), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+}
+
+// ----------------------------------------------------------------------------- eight neighbouring elements of a row, float or bfloat16
+// The bytes as they come from memory: converted where they are used, so that several loads are under way at once.
+struct Raw8 { uint4 a, b; };
+__device__ __forceinline__ Raw8 raw8_load(const void* row, int f32, int at) {
+    Raw8 r;
+    if (f32) {
+        const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(row) + at);
+        r.a = p[0];
+        r.b = p[1];
+    } else {
+        r.a = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(row) + at);
+        r.b = make_uint4(0, 0, 0, 0);
+    }
+    return r;
+}
+__device__ __forceinline__ void raw8_floats(const Raw8& r, int f32, float (&v)[8]) {
+    const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, b[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+    if (f32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[i] = __uint_as_float(a[i]);
+            v[4 + i] = __uint_as_float(b[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(a[i] << 16);
+            v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
+        }
+    }
+}
+// the same element by element, zeros from `n` on: for rows whose length, stride or start is not a multiple of 16 bytes
+__device__ __forceinline__ void load8_ragged(const void* row, int f32, int at, int n, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = at + i >= n ? 0.f : f32 ? reinterpret_cast<const float*>(row)[at + i] : __bfloat162float(reinterpret_cast<const bf16*>(row)[at + i]);
+}
+__device__ __forceinline__ void store8(void* row, int f32, int at, const float (&v)[8]) {
+    if (f32) {
+        float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(row) + at);
+        p[0] = make_float4(v[0], v[1], v[2], v[3]);
+        p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(row) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+__device__ __forceinline__ void store8_ragged(void* row, int f32, int at, int n, const float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (at + i < n) {
+            if (f32) reinterpret_cast<float*>(row)[at + i] = v[i];
+            else reinterpret_cast<bf16*>(row)[at + i] = __float2bfloat16_rn(v[i]);
+        }
+}
+template <bool VEC>
+__device__ __forceinline__ void store_q8(uint8_t* row, int at, int n, const float (&v)[8], float r) {
+    const uint32_t lo = fp8_pack4(v[0], v[1], v[2], v[3], r), hi = fp8_pack4(v[4], v[5], v[6], v[7], r);
+    if (VEC) {
+        *reinterpret_cast<uint2*>(row + at) = make_uint2(lo, hi);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (at + i < n) row[at + i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+    }
+}
+__device__ __forceinline__ uint32_t magnitude8(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, fp8_magnitude(v[i]));
+    return m;
+}
+// the largest over the sixteen lanes that hold a group of 128
+__device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+static inline bool fp8_rows_aligned(const void* p, long long ld, int bytes, int to) {
+    return !((uintptr_t)p % to) && !(ld * bytes % to);
+}

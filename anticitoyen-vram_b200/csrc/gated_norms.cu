@@ -1,0 +1,185 @@
+// The step between two parts of a layer: what the part before leaves joins the stream, and the part behind gets its norm.
+//
+//   n = d / sqrt(mean(d^2) + e1) * w1         (the norm behind the part; without w1 n = d)
+//   x += c * (g * n)                          (c: one number, g: a number for each channel or for each channel of each token)
+//   h = x / sqrt(mean(x^2) + e2) * w2         (the norm in front of the next part, of the stream as it is kept; optional)
+//
+// h is rounded once, to float, bfloat16, or e4m3 with a scale for each group of 128 (fp8.cuh), which is what an 8-bit product reads.
+// One block a row; a thread keeps its elements (eight neighbouring ones, C such pieces) in registers from their only read to their
+// only write, both statistics are 32-bit sums over the block.  Sixteen neighbouring lanes hold a group, so its maximum takes four
+// exchanges.  Memory bounds it with many rows, the chain load - sum - sum - store with few; the weights, which no kernel before
+// this one writes, are asked for before the wait for that kernel.
+#include "fp8.cuh"
+
+struct GnParams {
+    void* x;
+    const void *d, *g;
+    const float *w1, *w2, *gc;
+    void* out;
+    float* s;
+    long long ldx, ldd, ldg, ldo, lds;
+    int H, x_f32, d_f32, g_f32, out_kind;       // out_kind: 0 float, 1 bfloat16, 2 e4m3, 3 none
+    float c, e1, e2;
+};
+
+template <bool VEC>
+__device__ __forceinline__ void gn_load(const void* row, int f32, int at, int H, float (&v)[8]) {
+    if (VEC) raw8_floats(raw8_load(row, f32, at), f32, v);
+    else load8_ragged(row, f32, at, H, v);
+}
+
+// C: pieces of eight elements a thread.  With one piece the weights fit the registers beside it and are asked for early; with more
+// they are read where they are used.
+template <bool VEC, int C>
+__global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
+    __shared__ float red[32];
+    pdl_launch_dependents();
+    const int H = p.H;
+    float w1[8], w2[8], gc[8];
+    if (C == 1) {
+        const int at = threadIdx.x * 8;
+        if (at < H) {
+            if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
+            if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
+            if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
+        }
+    }
+    pdl_wait();
+    const size_t row = blockIdx.x;
+    char* xr = reinterpret_cast<char*>(p.x) + row * p.ldx * (p.x_f32 ? 4 : 2);
+    const char* dr = reinterpret_cast<const char*>(p.d) + row * p.ldd * (p.d_f32 ? 4 : 2);
+    const char* gr = p.g ? reinterpret_cast<const char*>(p.g) + row * p.ldg * (p.g_f32 ? 4 : 2) : nullptr;
+    Raw8 xw[C], dw[C], gw[C];
+    float x[C][8], d[C][8];
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            if (at < H) {
+                if (p.d) dw[i] = raw8_load(dr, p.d_f32, at);
+                xw[i] = raw8_load(xr, p.x_f32, at);
+                if (gr) gw[i] = raw8_load(gr, p.g_f32, at);
+            }
+        }
+    }
+    if (p.d) {
+        float r = 1.f;
+        if (p.w1) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < C; ++i) {
+                const int at = (threadIdx.x + i * blockDim.x) * 8;
+                if (at < H) {
+                    if (VEC) raw8_floats(dw[i], p.d_f32, d[i]);
+                    else load8_ragged(dr, p.d_f32, at, H, d[i]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ss = fmaf(d[i][e], d[i][e], ss);
+                }
+            }
+            ss = block_sum(ss, red);
+            r = 1.f / sqrtf(ss / (float)H + p.e1);
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            if (at >= H) continue;
+            if (p.w1) {
+                if (C > 1) gn_load<VEC>(p.w1, 1, at, H, w1);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[i][e] = d[i][e] * r * w1[e];
+            } else {
+                if (VEC) raw8_floats(dw[i], p.d_f32, d[i]);
+                else load8_ragged(dr, p.d_f32, at, H, d[i]);
+            }
+            if (gr) {
+                float g[8];
+                if (VEC) raw8_floats(gw[i], p.g_f32, g);
+                else load8_ragged(gr, p.g_f32, at, H, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[i][e] *= g[e];
+            } else if (p.gc) {
+                if (C > 1) gn_load<VEC>(p.gc, 1, at, H, gc);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d[i][e] *= gc[e];
+            }
+            if (VEC) raw8_floats(xw[i], p.x_f32, x[i]);
+            else load8_ragged(xr, p.x_f32, at, H, x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[i][e] = fmaf(p.c, d[i][e], x[i][e]);
+                if (!p.x_f32) x[i][e] = round_to<bf16>(x[i][e]);
+            }
+            if (VEC) store8(xr, p.x_f32, at, x[i]);
+            else store8_ragged(xr, p.x_f32, at, H, x[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            if (at >= H) continue;
+            if (VEC) raw8_floats(xw[i], p.x_f32, x[i]);
+            else load8_ragged(xr, p.x_f32, at, H, x[i]);
+        }
+    }
+    if (p.out_kind == 3) return;
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+        if ((threadIdx.x + i * blockDim.x) * 8 < H) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
+        }
+    ss = block_sum(ss, red);
+    const float r = 1.f / sqrtf(ss / (float)H + p.e2);
+    char* o = reinterpret_cast<char*>(p.out) + row * p.ldo * (p.out_kind == 0 ? 4 : p.out_kind == 1 ? 2 : 1);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int at = (threadIdx.x + i * blockDim.x) * 8;
+        const bool in = at < H;
+        if (C > 1 && in) gn_load<VEC>(p.w2, 1, at, H, w2);
+        float h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = (VEC ? in : at + e < H) ? x[i][e] * r * w2[e] : 0.f;      // (zeros behind the row's end)
+        if (p.out_kind == 2) {
+            const Fp8Scale k = fp8_scale(half_warp_max(magnitude8(h)));      // (whole warps pass here)
+            if (in) {
+                store_q8<VEC>(reinterpret_cast<uint8_t*>(o), at, H, h, k.r);
+                if ((threadIdx.x & 15) == 0) p.s[row * p.lds + at / FP8_GROUP] = k.s;
+            }
+        } else if (in) {
+            if (VEC) store8(o, p.out_kind == 0, at, h);
+            else store8_ragged(o, p.out_kind == 0, at, H, h);
+        }
+    }
+}
+
+template <bool VEC>
+static int gn_launch(const GnParams& p, int T, cudaStream_t stream) {
+    const int pieces = (p.H + 7) / 8;
+    auto threads = [&](int c) { return ((pieces + c - 1) / c + 31) / 32 * 32; };
+    if (threads(1) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 1>, T, threads(1), 0, stream, p);
+    else if (threads(2) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 2>, T, threads(2), 0, stream, p);
+    else if (threads(4) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 4>, T, threads(4), 0, stream, p);
+    else return ACV_ERR_SIZE;
+    return acv_launch_status();
+}
+
+// x [T,H] in place; d [T,H] or null; gate: g [T,H] or gc float [H] or neither; w1 or null; out [T,H] of out_dtype (0 float, 1
+// bfloat16, 2 e4m3 with scales s [T][groups of H]) or null; every matrix's rows dense at a stride of its own.
+ACV_API int acv_add_gated_norms(void* x, int x_dtype, long long ldx, const void* d, int d_dtype, long long ldd, const void* g, int g_dtype,
+                                long long ldg, const float* gc, const float* w1, float e1, float c, const float* w2, float e2, void* out,
+                                int out_dtype, long long ldo, float* s, long long lds, int T, int H, cudaStream_t stream) {
+    if (T <= 0 || H <= 0) return 0;
+    if ((x_dtype | d_dtype | g_dtype) & ~1) return ACV_ERR_DTYPE;
+    if (out && ((unsigned)out_dtype > 2u || !w2 || (out_dtype == 2 && !s))) return ACV_ERR_DTYPE;
+    GnParams p = {};
+    p.x = x; p.d = d; p.g = g; p.gc = g ? nullptr : gc; p.w1 = d ? w1 : nullptr; p.w2 = out ? w2 : nullptr; p.out = out; p.s = s;
+    p.ldx = ldx; p.ldd = ldd; p.ldg = ldg; p.ldo = ldo; p.lds = lds; p.H = H;
+    p.x_f32 = x_dtype == ACV_F32; p.d_f32 = d_dtype == ACV_F32; p.g_f32 = g_dtype == ACV_F32; p.out_kind = out ? out_dtype : 3;
+    p.c = c; p.e1 = e1; p.e2 = e2;
+    const int ob = p.out_kind == 0 ? 4 : p.out_kind == 1 ? 2 : 1;
+    const bool vec = H % 8 == 0 && fp8_rows_aligned(x, ldx, p.x_f32 ? 4 : 2, 16) && (!d || fp8_rows_aligned(d, ldd, p.d_f32 ? 4 : 2, 16)) &&
+                     (!g || fp8_rows_aligned(g, ldg, p.g_f32 ? 4 : 2, 16)) && (!out || fp8_rows_aligned(out, ldo, ob, p.out_kind == 2 ? 8 : 16)) &&
+                     !(((uintptr_t)p.gc | (uintptr_t)p.w1 | (uintptr_t)p.w2) & 15);
+    return vec ? gn_launch<true>(p, T, stream) : gn_launch<false>(p, T, stream);
+}

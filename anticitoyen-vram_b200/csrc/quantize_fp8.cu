@@ -1,0 +1,127 @@
+// Quantisation to e4m3: rows in groups of 128 (what a product's activations are) and blocks of 128 x 128 (its weights).
+// The formulas stand in fp8.cuh.  Both forms read every element once and write a byte for it: memory bounds them.
+#include "fp8.cuh"
+
+// Rows: sixteen lanes hold a group, eight neighbouring elements each, so the group's maximum takes four exchanges and no shared
+// memory.  A half-warp takes U groups at once, their loads in flight together, and goes on by the grid's stride; the stride in
+// (rows, groups) comes from the host, so no group costs a division.
+template <bool VEC, int U>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int f32, long long ldx, uint8_t* __restrict__ q,
+                                                            long long ldq, float* __restrict__ s, long long lds, int T, int K, int G,
+                                                            int step_rows, int step_groups) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int lane = threadIdx.x & 15;
+    const size_t esz = f32 ? 4 : 2;
+    const long long first = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    int row = (int)(first / G), g = (int)(first - (long long)row * G);
+    // (a warp's halves leave the loop together: the exchanges are the whole warp's)
+    while (__any_sync(0xffffffffu, row < T)) {
+        int rows[U], gs[U];
+        Raw8 raw[U];
+        float v[U][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            rows[u] = row;
+            gs[u] = g;
+            row += step_rows;
+            g += step_groups;
+            if (g >= G) { g -= G; ++row; }
+            const int at = gs[u] * FP8_GROUP + lane * 8;
+            const bool in = rows[u] < T && at < K;
+            const char* src = reinterpret_cast<const char*>(x) + (size_t)rows[u] * ldx * esz;
+            if (VEC) {
+                raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
+                if (in) raw[u] = raw8_load(src, f32, at);
+            } else {
+                load8_ragged(src, f32, at, in ? K : 0, v[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (VEC) raw8_floats(raw[u], f32, v[u]);
+            const Fp8Scale k = fp8_scale(half_warp_max(magnitude8(v[u])));
+            const int at = gs[u] * FP8_GROUP + lane * 8;
+            if (rows[u] < T) {
+                if (at < K) store_q8<VEC>(q + (size_t)rows[u] * ldq, at, K, v[u], k.r);
+                if (lane == 0) s[(size_t)rows[u] * lds + gs[u]] = k.s;
+            }
+        }
+    }
+}
+
+// Blocks: 256 threads hold a block of 128 x 128 in registers (eight rows of eight elements a thread) between its maximum and its
+// quantised values, so it is read once.
+template <bool VEC>
+__global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __restrict__ x, int f32, long long ldx, uint8_t* __restrict__ q,
+                                                              long long ldq, float* __restrict__ s, long long lds, int T, int K) {
+    __shared__ uint32_t red[8];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int at = blockIdx.x * FP8_GROUP + (threadIdx.x & 15) * 8;
+    const int row0 = blockIdx.y * FP8_GROUP + (threadIdx.x >> 4);
+    const size_t esz = f32 ? 4 : 2;
+    Raw8 raw[8];
+    float v[8];
+    uint32_t m = 0;
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            raw[i].a = raw[i].b = make_uint4(0, 0, 0, 0);
+            if (row0 + 16 * i < T && at < K)
+                raw[i] = raw8_load(reinterpret_cast<const char*>(x) + (size_t)(row0 + 16 * i) * ldx * esz, f32, at);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (VEC) raw8_floats(raw[i], f32, v);
+        else load8_ragged(reinterpret_cast<const char*>(x) + (size_t)(row0 + 16 * i) * ldx * esz, f32, at, row0 + 16 * i < T ? K : 0, v);
+        m = max(m, magnitude8(v));
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+    const Fp8Scale k = fp8_scale(m);
+    if (threadIdx.x == 0) s[(size_t)blockIdx.y * lds + blockIdx.x] = k.s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = row0 + 16 * i;
+        if (row >= T || at >= K) continue;
+        if (VEC) raw8_floats(raw[i], f32, v);
+        else load8_ragged(reinterpret_cast<const char*>(x) + (size_t)row * ldx * esz, f32, at, K, v);
+        store_q8<VEC>(q + (size_t)row * ldq, at, K, v, k.r);
+    }
+}
+
+// x [T,K] float or bfloat16, rows dense at stride ldx; q [T,K] bytes at stride ldq; s: block_rows 1: [T][groups of K] at stride lds,
+// 128: [blocks of T][groups of K].
+ACV_API int acv_quantize_fp8(const void* x, int dtype, long long ldx, void* q, long long ldq, float* s, long long lds, int T, int K,
+                             int block_rows, int sms, cudaStream_t stream) {
+    if (T <= 0 || K <= 0) return 0;
+    if (dtype != ACV_F32 && dtype != ACV_BF16) return ACV_ERR_DTYPE;
+    const int f32 = dtype == ACV_F32;
+    const int G = (K + FP8_GROUP - 1) / FP8_GROUP;
+    const bool vec = K % 8 == 0 && fp8_rows_aligned(x, ldx, f32 ? 4 : 2, 16) && fp8_rows_aligned(q, ldq, 1, 8);
+    if (block_rows == FP8_GROUP) {
+        const long long down = ((long long)T + FP8_GROUP - 1) / FP8_GROUP;
+        if (down > 65535) return ACV_ERR_SIZE;
+        const dim3 grid(G, (unsigned)down);
+        if (vec) acv_launch(PDL_MISC, quantize_blocks_kernel<true>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K);
+        else acv_launch(PDL_MISC, quantize_blocks_kernel<false>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K);
+        return acv_launch_status();
+    }
+    if (block_rows != 1) return ACV_ERR_SIZE;
+    const long long groups = (long long)T * G;
+    const long long blocks = (groups + 15) / 16;
+    const int grid = (int)(blocks < (long long)sms * 8 ? blocks : (long long)sms * 8);
+    const long long stride = (long long)grid * 16;
+    const int step_rows = (int)(stride / G), step_groups = (int)(stride % G);
+    if ((long long)T + 4ll * (step_rows + 1) > 0x7fffffffll) return ACV_ERR_SIZE;
+    if (!vec)
+        acv_launch(PDL_MISC, quantize_rows_kernel<false, 1>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K, G, step_rows, step_groups);
+    else
+        acv_launch(PDL_MISC, quantize_rows_kernel<true, 4>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K, G, step_rows, step_groups);
+    return acv_launch_status();
+}

@@ -146,6 +146,10 @@ def _declare(lib: ctypes.CDLL) -> None:
         "acv_moe_combine": [P, I, I, P, I, P, I, P, P, I, I, I, I, P],
         "acv_glu": [P, I, P, I, I, I, I, F, F, I, I, P],
         "acv_gemm_tc_glu": [P, I, P, I, P, I, I, I, I, F, F, I, P, I, I, I, P],
+        "acv_quantize_fp8": [P, I, LL, P, LL, P, LL, I, I, I, I, P],
+        "acv_add_gated_norms": [P, I, LL, P, I, LL, P, I, LL, P, P, F, F, P, F, P, I, LL, P, LL, I, I, P],
+        "acv_gemm_fp8_rows": [P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, I, P],
+        "acv_gemm_fp8_rows_gated": [P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, P],
         "acv_argmax": [P, I, I, I, P, P],
         "acv_apply_penalties": [P, I, I, P, P, P, I, P, P, P, P],
         "acv_sample": [P, I, I, I, P, P, P, P, P, P, P, P, P],
@@ -2363,3 +2367,150 @@ def gated_delta(proj: torch.Tensor, taps_t: torch.Tensor, rate: torch.Tensor, sh
     o = torch.empty((T, I), device=proj.device, dtype=torch.float32)
     delta(rec, values, state, slots, cu_q, num_seqs, o, num_heads, dim, work, value_dim=value_dim, gated=True)
     return retention_gate(o, proj[:, C:C + I], out, num_heads, value_dim, eps, weight=weight, gate_fn="silu")
+
+
+# ----------------------------------------------------------------------------- 8-bit floats with block scales
+# A quantised matrix is a pair: values float8_e4m3fn [R, C] and scales float32, one for each group of 128 neighbouring elements of a
+# row ([R, groups], activations) or for each block of 128 x 128 elements ([blocks of R, groups], weights).  It stands for value * scale.
+FP8 = torch.float8_e4m3fn
+FP8_GROUP = 128
+
+
+def fp8_rows(rows: int, columns: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Uninitialised (values, scales) of a matrix quantised in groups of a row; a row's stride is a multiple of 16 bytes, as the
+    products ask for."""
+    values = torch.empty((rows, (columns + 15) // 16 * 16), device=device, dtype=FP8)[:, :columns]
+    return values, torch.empty((rows, (columns + 127) // 128), device=device, dtype=torch.float32)
+
+
+def _one_device(name: str, *tensors) -> int:
+    """The device that all of them lie on."""
+    device = tensors[0].get_device()
+    if device < 0:
+        raise KernelError("acvram_b200 kernels run on a CUDA device only; got a CPU tensor")
+    for t in tensors:
+        if t is not None and t.get_device() != device:
+            raise KernelError(f"{name}: the tensors lie on different devices")
+    return device
+
+
+def _launch_on(device: int, name: str, entry, *args) -> None:
+    """Launch on that device's current stream, whichever device is current."""
+    if device == torch._C._cuda_getDevice():
+        _check(entry(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+    else:
+        with torch.cuda.device(device):
+            _check(entry(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+
+
+def _fp8_pair(name: str, what: str, values: torch.Tensor, scales: torch.Tensor, rows: int, columns: int, block_rows: int) -> None:
+    """Raises unless (values, scales) are a quantised matrix of that size with dense rows."""
+    if values.dtype != FP8 or values.shape != (rows, columns) or (values.stride(1) != 1 and columns > 1):
+        raise KernelError(f"{name}: {what} must be float8_e4m3fn [{rows}, {columns}] with dense rows, got {values.dtype} "
+                          f"{list(values.shape)} strides {values.stride()}")
+    want = (rows if block_rows == 1 else (rows + 127) // 128, (columns + 127) // 128)
+    if scales.dtype != torch.float32 or scales.shape != want or (scales.stride(1) != 1 and want[1] > 1):
+        raise KernelError(f"{name}: the scales of {what} must be float32 {list(want)} with dense rows, got {scales.dtype} "
+                          f"{list(scales.shape)} strides {scales.stride()}")
+
+
+def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
+    """(values, scales) of x [R, C] (float32 or bfloat16, dense rows at any stride), in groups of 128 of a row (``block_rows`` 1) or
+    in blocks of 128 x 128 (``block_rows`` 128): s = max(largest magnitude / 448, 2^-126), value = e4m3(x * (1 / s)), each step
+    rounded once.  A group with a NaN becomes NaN as a whole; one with an infinity gets an infinite scale."""
+    if x.dim() != 2 or block_rows not in (1, 128):
+        raise KernelError("quantize_fp8: a matrix, and block_rows 1 or 128, are wanted")
+    R, C = x.shape
+    if x.stride(1) != 1 and C > 1:
+        raise KernelError("quantize_fp8: the rows of x must be dense")
+    _fp8_pair("quantize_fp8", "the result", values, scales, R, C, block_rows)
+    device = _one_device("quantize_fp8", x, values, scales)
+    if R and C:
+        _launch_on(device, "quantize_fp8", library().acv_quantize_fp8, x.data_ptr(), dtype_code(x.dtype), x.stride(0), values.data_ptr(),
+                   values.stride(0), scales.data_ptr(), scales.stride(0), R, C, block_rows, sm_count(x.device))
+    return values, scales
+
+
+def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    """out[T, N] = x @ w^T of quantised matrices: x [T, K] with a scale for each group of 128 of a row, w [N, K] with a scale for each
+    block of 128 x 128; out float32 or bfloat16, dense rows at any stride.  A group's sum is multiplied by its two scales in float
+    and joins a float sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``)."""
+    T, K = x.shape
+    N = w.shape[0]
+    _fp8_pair("linear_fp8", "x", x, x_scales, T, K, 1)
+    _fp8_pair("linear_fp8", "w", w, w_scales, N, K, 128)
+    if out.shape != (T, N) or (out.stride(1) != 1 and N > 1):
+        raise KernelError(f"linear_fp8: out must be [{T}, {N}] with dense rows, got {list(out.shape)} strides {out.stride()}")
+    device = _one_device("linear_fp8", x, x_scales, w, w_scales, out)
+    if not T or not N:
+        return out
+    if not K:
+        return out.zero_()
+    _launch_on(device, "linear_fp8", library().acv_gemm_fp8_rows, x.data_ptr(), x.stride(0), x_scales.data_ptr(), x_scales.stride(0),
+               w.data_ptr(), w.stride(0), w_scales.data_ptr(), w_scales.stride(0), out.data_ptr(), out.stride(0),
+               1 if dtype_code(out.dtype) == F32 else 0, T, N, K, 1, sm_count(x.device))
+    return out
+
+
+def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor,
+                      up_scales: torch.Tensor, out: torch.Tensor, out_scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out, out_scales) = silu(x @ gate^T) * (x @ up^T), quantised in groups of 128 units: what the next ``linear_fp8`` reads.
+    Operands as there, gate and up [I, K] each with its own scales.  Unit and quantisation are float, from the float sums."""
+    T, K = x.shape
+    I = gate.shape[0]
+    _fp8_pair("linear_fp8_swiglu", "x", x, x_scales, T, K, 1)
+    _fp8_pair("linear_fp8_swiglu", "gate", gate, gate_scales, I, K, 128)
+    _fp8_pair("linear_fp8_swiglu", "up", up, up_scales, I, K, 128)
+    _fp8_pair("linear_fp8_swiglu", "the result", out, out_scales, T, I, 1)
+    device = _one_device("linear_fp8_swiglu", x, x_scales, gate, gate_scales, up, up_scales, out, out_scales)
+    if not T or not I:
+        return out, out_scales
+    if not K:
+        raise KernelError("linear_fp8_swiglu: K is 0")
+    _launch_on(device, "linear_fp8_swiglu", library().acv_gemm_fp8_rows_gated, x.data_ptr(), x.stride(0), x_scales.data_ptr(),
+               x_scales.stride(0), gate.data_ptr(), gate.stride(0), gate_scales.data_ptr(), gate_scales.stride(0), up.data_ptr(),
+               up.stride(0), up_scales.data_ptr(), up_scales.stride(0), out.data_ptr(), out.stride(0), out_scales.data_ptr(),
+               out_scales.stride(0), T, I, K, 1, sm_count(x.device))
+    return out, out_scales
+
+
+_NORM_OUT = {torch.float32: 0, torch.bfloat16: 1, FP8: 2}
+
+
+def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tensor | None, out_scales: torch.Tensor | None = None, *,
+                    post_weight: torch.Tensor | None = None, post_eps: float = 0.0, gate: torch.Tensor | None = None,
+                    residual_scale: float = 1.0, weight: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor | None:
+    """The stream x [T, H] += residual_scale * gate * n, in place, n = delta / sqrt(mean(delta^2) + post_eps) * post_weight (without
+    ``post_weight``: n = delta); then, with ``out``, out = x / sqrt(mean(x^2) + eps) * weight of the stream as it is kept.
+
+    x and delta float32 or bfloat16; ``gate`` float32 [H], or [T, H] float32 or bfloat16; weights float32 [H].  out float32 or
+    bfloat16, rounded once, or float8_e4m3fn with ``out_scales``: quantised in groups of 128 as ``quantize_fp8`` does.  Matrices
+    have dense rows at any stride; H up to 16384.  Sums and both statistics are 32-bit."""
+    T, H = x.shape
+    for t in (x, delta, gate if gate is not None and gate.dim() == 2 else None, out):
+        if t is not None and (t.shape != x.shape or (t.stride(1) != 1 and H > 1)):
+            raise KernelError("add_gated_norms: delta, a gate by tokens and out are of the stream's shape, all with dense rows")
+    vector = gate if gate is not None and gate.dim() != 2 else None
+    for v in (post_weight, weight, vector):
+        if v is not None and (v.dtype != torch.float32 or v.shape != (H,) or (v.stride(0) != 1 and H > 1)):
+            raise KernelError("add_gated_norms: weights and a gate by channels are dense float32 vectors of the stream's width")
+    if delta is None and (gate is not None or post_weight is not None):
+        raise KernelError("add_gated_norms: a gate or a norm behind the part, but no delta")
+    kind = 3
+    if out is not None:
+        kind = _NORM_OUT.get(out.dtype, 3)
+        if kind == 3 or weight is None or (kind == 2) != (out_scales is not None):
+            raise KernelError("add_gated_norms: out is float32, bfloat16, or float8_e4m3fn with out_scales, and wants a weight")
+        if kind == 2:
+            _fp8_pair("add_gated_norms", "out", out, out_scales, T, H, 1)
+    elif out_scales is not None:
+        raise KernelError("add_gated_norms: scales without a result")
+    device = _one_device("add_gated_norms", x, delta, gate, post_weight, weight, out, out_scales)
+    if T and H:
+        rows = gate if vector is None else None
+        _launch_on(device, "add_gated_norms", library().acv_add_gated_norms, x.data_ptr(), dtype_code(x.dtype), x.stride(0), _p(delta),
+                   0 if delta is None else dtype_code(delta.dtype), 0 if delta is None else delta.stride(0), _p(rows),
+                   0 if rows is None else dtype_code(rows.dtype), 0 if rows is None else rows.stride(0), _p(vector), _p(post_weight),
+                   post_eps, residual_scale, _p(weight), eps, _p(out), kind if kind < 3 else 0, 0 if out is None else out.stride(0),
+                   _p(out_scales), 0 if out_scales is None else out_scales.stride(0), T, H)
+    return out

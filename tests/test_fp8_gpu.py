@@ -1,0 +1,277 @@
+"""The 8-bit operators against plain forms: quantisation bit for bit, products and norms within bounds that count roundings."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import plain_fp8 as pf
+from plain_fp8 import EPS32, FP8, groups
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def ops():
+    from acvram_b200.kernels import ops as module
+    return module
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def activations(T, K, seed, dtype=F32):
+    g = gen(seed)
+    x = torch.randn((T, K), generator=g) * (0.3 + 2 * torch.rand((T, 1), generator=g))
+    x[:, torch.randint(0, K, (1 + K // 200,), generator=g)] *= 20.0
+    return x.to(dtype)
+
+
+def device_pair(q, s, pad=0):
+    """A quantised matrix on the device, rows at a stride of a multiple of 16 bytes and `pad` more."""
+    R, C = q.shape
+    buf = torch.full((R, (C + 15) // 16 * 16 + pad), 0x55, dtype=torch.uint8, device=DEV)
+    buf[:, :C] = q.view(torch.uint8).to(DEV)
+    return buf.view(FP8)[:, :C], s.to(DEV)
+
+
+def quantized(R, C, seed, block_rows, factor=1.0, pad=0):
+    q, s = pf.quantize(activations(R, C, seed) * factor, block_rows)
+    return device_pair(q, s, pad)
+
+
+def same_bits(a, b):
+    a, b = a.cpu().view(torch.uint8), b.cpu().view(torch.uint8)
+    nan = ((a & 0x7f) == 0x7f) & ((b & 0x7f) == 0x7f)
+    return bool(((a == b) | nan).all())
+
+
+# ----------------------------------------------------------------------------- quantisation
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("R,C", [(1, 1), (1, 128), (3, 7), (5, 130), (64, 96), (129, 264), (130, 1100), (257, 2048), (7, 12288), (2, 20001)])
+def test_quantize_is_exact(R, C, block_rows, dtype):
+    x = activations(R, C, R * 1000 + C, dtype)
+    q, s = ops().fp8_rows(R, C, DEV)
+    if block_rows == 128:
+        s = torch.empty((groups(R), groups(C)), device=DEV)
+    ops().quantize_fp8(x.to(DEV), q, s, block_rows)
+    want_q, want_s = pf.quantize(x.float(), block_rows)
+    assert torch.equal(s.cpu(), want_s)
+    assert same_bits(q, want_q)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("offset,stride", [(0, 400), (1, 401), (8, 264), (16, 272)])
+def test_quantize_views_leave_their_surroundings(block_rows, offset, stride):
+    R, C = 37, 200
+    base = torch.full((R + 2, stride), 7.0, dtype=BF, device=DEV)
+    x = base[1:R + 1, offset:offset + C]
+    x.copy_(activations(R, C, 5, BF))
+    buf = torch.full((R + 2, stride + 3), 0x55, dtype=torch.uint8, device=DEV)
+    q = buf.view(FP8)[1:R + 1, offset:offset + C]
+    down = R if block_rows == 1 else 1
+    sbuf = torch.full((down + 2, 5), 3.0, device=DEV)
+    s = sbuf[1:down + 1, 1:3]
+    ops().quantize_fp8(x, q, s, block_rows)
+    want_q, want_s = pf.quantize(x.cpu().float(), block_rows)
+    assert torch.equal(s.cpu(), want_s) and same_bits(q.contiguous(), want_q)
+    buf.view(FP8)[1:R + 1, offset:offset + C].view(torch.uint8).fill_(0x55)
+    s.fill_(3.0)
+    assert bool((buf == 0x55).all()) and bool((sbuf == 3.0).all())
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_quantize_of_values_at_the_edges(block_rows, dtype):
+    x = activations(6 if block_rows == 1 else 6 * 128, 384, 11)
+    step = 1 if block_rows == 1 else 128
+    x[0 * step:1 * step] = 0.0
+    x[1 * step] = 1e-40                                     # under the smallest normal float
+    x[2 * step, 130] = float("inf")
+    x[3 * step, 5] = float("nan")
+    x[4 * step] = torch.finfo(dtype).max
+    x[5 * step, 200] = -float("inf")
+    x = x.to(dtype)
+    q, s = ops().fp8_rows(*x.shape, DEV)
+    if block_rows == 128:
+        s = torch.empty((groups(x.shape[0]), 3), device=DEV)
+    ops().quantize_fp8(x.to(DEV), q, s, block_rows)
+    want_q, want_s = pf.quantize(x.float(), block_rows)
+    assert torch.equal(torch.nan_to_num(s.cpu(), nan=-1.0), torch.nan_to_num(want_s, nan=-1.0))
+    assert same_bits(q, want_q)
+
+
+# ----------------------------------------------------------------------------- the product
+def check_product(T, N, K, out_dtype, seed, pads=(0, 0, 0)):
+    x, xs = quantized(T, K, seed, 1, pad=16 * pads[0])
+    w, ws = quantized(N, K, seed + 1, 128, 0.02, pad=16 * pads[1])
+    buf = torch.full((T + 1, N + 1 + pads[2]), 7.0, dtype=out_dtype, device=DEV)
+    out = buf[:T, :N]
+    assert ops().linear_fp8(x, xs, w, ws, out) is out
+    want, error = pf.product(x, xs, w, ws)
+    if out_dtype != F32:
+        error = error + pf.half_step(want.abs() + error, out_dtype)
+    else:
+        error = error + pf.half_step(want, F32)
+    off = (out.cpu().double() - want).abs()
+    assert bool((off <= error).all()), float((off / error).max())
+    assert bool((buf[T:] == 7.0).all()) and bool((buf[:, N:] == 7.0).all())
+
+
+@pytest.mark.parametrize("out_dtype", [BF, F32])
+@pytest.mark.parametrize("T", [1, 2, 7, 8, 9, 16, 17, 33, 64, 65, 100, 128, 129, 200, 257, 300, 520])
+@pytest.mark.parametrize("N,K", [(128, 128), (136, 144), (1000, 1104), (257, 2048)])
+def test_product(T, N, K, out_dtype):
+    check_product(T, N, K, out_dtype, T * 7 + N)
+
+
+@pytest.mark.parametrize("T,N,K", [(1, 1, 16), (1, 5, 1), (3, 16, 100), (9, 31, 48), (1, 4096, 4096), (8, 640, 12288), (16, 1024, 5120),
+                                   (40, 7, 4096), (130, 1, 256), (70, 130, 17408), (600, 2049, 272), (1024, 520, 640), (2050, 384, 512)])
+def test_product_of_other_sizes(T, N, K):
+    check_product(T, N, K, F32, T + N + K, (1, 2, 3))
+
+
+@pytest.mark.parametrize("T", [1, 12, 90, 400])
+def test_product_of_values_that_are_no_numbers(T):
+    """A NaN or an infinity in a token's group, or an infinite scale, reaches that token's outputs and no other's."""
+    N, K = 200, 400
+    a = activations(T, K, 3)
+    if T > 2:
+        a[1, 300] = float("inf")
+        a[T - 1, 2] = float("nan")
+    x, xs = device_pair(*pf.quantize(a, 1))
+    w, ws = quantized(N, K, 4, 128, 0.02)
+    out = torch.empty((T, N), device=DEV)
+    ops().linear_fp8(x, xs, w, ws, out)
+    bad = torch.isnan(out).all(1).cpu()
+    some = torch.isnan(out).any(1).cpu()
+    want = torch.zeros(T, dtype=torch.bool)
+    if T > 2:
+        want[1] = want[T - 1] = True
+    assert torch.equal(bad, want) and torch.equal(some, want)
+
+
+# ----------------------------------------------------------------------------- the product with the gated unit
+def check_gated(T, I, K, seed, gate_factor=0.05):
+    x, xs = quantized(T, K, seed, 1)
+    g, gs = quantized(I, K, seed + 1, 128, gate_factor)
+    u, us = quantized(I, K, seed + 2, 128, 0.02)
+    buf = torch.full((T + 1, (I + 15) // 16 * 16 + 16), 0x55, dtype=torch.uint8, device=DEV)
+    out = buf.view(FP8)[:T, :I]
+    sbuf = torch.full((T + 1, groups(I) + 1), 3.0, device=DEV)
+    scales = sbuf[:T, :groups(I)]
+    ops().linear_fp8_swiglu(x, xs, g, gs, u, us, out, scales)
+    yg, eg = pf.product(x, xs, g, gs)
+    yu, eu = pf.product(x, xs, u, us)
+    h = yg * torch.sigmoid(yg) * yu
+    # the unit's slope is at most 1.1; the exponential, the quotient and the product are a few units of a float
+    error = 1.1 * eg * (yu.abs() + eu) + (yg * torch.sigmoid(yg)).abs() * eu + h.abs() * 16 * EPS32
+    off = (pf.values(out, scales, 1) - h).abs()
+    bound = pf.quantized_error(h, scales, error)
+    assert bool((off <= bound).all()), float((off / bound).max())
+    pad = groups(I) * 128 - I
+    most = torch.nn.functional.pad(h.abs(), (0, pad)).view(T, -1, 128).amax(2) / 448
+    most_error = torch.nn.functional.pad(error, (0, pad)).view(T, -1, 128).amax(2) / 448
+    assert bool(((scales.cpu().double() - most).abs() <= most_error + most * 2 * EPS32 + 2.0 ** -126).all())
+    assert bool((buf[T:] == 0x55).all()) and bool((buf[:, I:] == 0x55).all())
+    assert bool((sbuf[T:] == 3.0).all()) and bool((sbuf[:, groups(I):] == 3.0).all())
+
+
+@pytest.mark.parametrize("T", [1, 5, 8, 9, 16, 17, 40, 64, 65, 128, 129, 300])
+@pytest.mark.parametrize("I,K", [(128, 128), (200, 144), (1, 16), (1030, 1104), (640, 2048)])
+def test_gated_product(T, I, K):
+    check_gated(T, I, K, T + I)
+
+
+@pytest.mark.parametrize("T,I,K", [(1, 4096, 4096), (4, 300, 12288), (70, 130, 5120), (520, 2049, 272), (1030, 384, 640)])
+def test_gated_product_of_other_sizes(T, I, K):
+    check_gated(T, I, K, T + I + K)
+
+
+# ----------------------------------------------------------------------------- the norms
+def check_norms(T, H, stream, delta, post, gate, out_dtype, seed=0, views=False):
+    g = gen(seed + T * 31 + H)
+    def matrix(values, dtype, extra):
+        if not views:
+            return values.to(dtype).to(DEV)
+        buf = torch.full((T, H + extra), 9.0, dtype=dtype, device=DEV)
+        buf[:, :H] = values.to(dtype)
+        return buf[:, :H]
+    x = matrix(3 * activations(T, H, seed + 1), stream, 24)
+    d = matrix(0.5 * activations(T, H, seed + 2), delta, 8) if delta is not None else None
+    w1 = (1 + 0.2 * torch.randn(H, generator=g)).to(DEV) if post else None
+    w2 = (1 + 0.2 * torch.randn(H, generator=g)).to(DEV)
+    gv = None
+    if gate == "channels":
+        gv = torch.randn(H, generator=g).to(DEV)
+    elif gate is not None:
+        gv = matrix(torch.randn((T, H), generator=g), gate, 16)
+    c = 0.7
+    x0 = x.cpu().double()
+    if out_dtype == FP8:
+        out, scales = ops().fp8_rows(T, H, DEV)
+    else:
+        out, scales = (torch.empty((T, H), dtype=out_dtype, device=DEV) if out_dtype is not None else None), None
+    ops().add_gated_norms(x, d, out, scales, post_weight=w1, post_eps=1e-5, gate=gv, residual_scale=c,
+                          weight=w2 if out is not None else None, eps=1e-6)
+    # a sum of H squares by a thread's sixteen to 64 and then by ten halvings: at most 80 roundings, half of which the root keeps;
+    # the products in front of and behind it are six more
+    rounds = 50 * EPS32
+    want = x0
+    error = torch.zeros_like(x0)
+    if d is not None:
+        n = d.cpu().double()
+        if w1 is not None:
+            n = n / torch.sqrt(n.square().mean(1, keepdim=True) + 1e-5) * w1.cpu().double()
+        if gv is not None:
+            n = n * gv.cpu().double()
+        want = x0 + c * n
+        error = (c * n).abs() * rounds + (want.abs() + (c * n).abs() * rounds) * EPS32
+        if stream != F32:
+            error = error + pf.half_step(want.abs() + error, stream)
+    kept = x.cpu().double()
+    assert bool(((kept - want).abs() <= error).all())
+    if out is None:
+        return
+    h = kept / torch.sqrt(kept.square().mean(1, keepdim=True) + 1e-6) * w2.cpu().double()
+    error = h.abs() * rounds
+    if out_dtype == FP8:
+        off, bound = (pf.values(out, scales, 1) - h).abs(), pf.quantized_error(h, scales, error)
+        most = torch.nn.functional.pad(h.abs(), (0, groups(H) * 128 - H)).view(T, -1, 128).amax(2) / 448
+        assert bool(((scales.cpu().double() - most).abs() <= most * (rounds + 2 * EPS32) + 2.0 ** -126).all())
+    else:
+        off, bound = (out.cpu().double() - h).abs(), error + pf.half_step(h.abs() + error, out_dtype)
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF, FP8, None])
+@pytest.mark.parametrize("stream", [F32, BF])
+@pytest.mark.parametrize("T,H", [(1, 1), (3, 96), (2, 127), (5, 1024), (8, 4096), (3, 5120), (2, 8200), (2, 16384)])
+def test_norms(T, H, stream, out_dtype):
+    check_norms(T, H, stream, BF, True, None, out_dtype)
+
+
+@pytest.mark.parametrize("views", [False, True])
+@pytest.mark.parametrize("gate", [None, "channels", F32, BF])
+@pytest.mark.parametrize("delta,post", [(F32, False), (F32, True), (BF, False), (BF, True)])
+def test_norms_with_gates(delta, post, gate, views):
+    check_norms(6, 1032, F32, delta, post, gate, FP8, 3, views)
+    check_norms(4, 203, BF, delta, post, gate, BF, 4, views)
+
+
+@pytest.mark.parametrize("out_dtype", [F32, BF, FP8])
+def test_norm_without_a_part(out_dtype):
+    check_norms(5, 640, BF, None, False, None, out_dtype)
+    check_norms(5, 6000, F32, None, False, None, out_dtype)
+
+
+def test_norms_of_rows_of_zeros():
+    H = 256
+    x, d = torch.zeros((2, H), device=DEV), torch.zeros((2, H), device=DEV)
+    w = torch.ones(H, device=DEV)
+    q, s = ops().fp8_rows(2, H, DEV)
+    ops().add_gated_norms(x, d, q, s, post_weight=w, post_eps=1e-6, weight=w, eps=1e-6)
+    assert bool((x == 0).all()) and bool((q.float() == 0).all()) and bool((s == 2.0 ** -126).all())
