@@ -7,15 +7,11 @@
 // alone reads, so no barrier stands in the loop: a group of a row is 128 bytes, as 64 bfloat16 are, and the ring's layout is the same.
 // Which k of a group a lane holds is the same for tokens and weights.
 #include "fp8.cuh"
+#include "gemm_fp8.h"
 #include "rows_ring.cuh"
 
-struct Fp8RowsParams {
-    const uint8_t *x, *w, *w2;          // w2: the up rows of the gated form
-    const float *sx, *sw, *sw2;
-    void* out;
-    float* so;                          // gated: the scales of the quantised result
-    long long ldx, ldw, ldw2, ldo, ldsx, ldsw, ldsw2, ldso;
-    int M, N, K, G, out_f32, early_w;
+struct Fp8RowsParams : Fp8Operands {
+    int G, early_w;                     // groups of K; the weights may be read before the kernel in front has ended
 };
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -306,38 +302,12 @@ static int fg_launch(const Fp8RowsParams& p, cudaStream_t stream) {
     return acv_launch_status();
 }
 
-static int fr_checks(const Fp8RowsParams& p) {
-    if (((uintptr_t)p.x | (uintptr_t)p.w | (uintptr_t)p.w2) % 16 || (p.ldx | p.ldw | p.ldw2) % 16) return ACV_ERR_ALIGN;
+int acv_fp8_rows(const Fp8Operands& o, int flags, int sms, cudaStream_t stream) {
+    Fp8RowsParams p = {};
+    static_cast<Fp8Operands&>(p) = o;
+    p.G = (p.K + FP8_GROUP - 1) / FP8_GROUP;
+    p.early_w = flags & 1;
     if ((p.M + 7) / 8 > 65535) return ACV_ERR_SIZE;
-    return 0;
-}
-
-// x [M,K] bytes, sx [M][groups of K]; w [N,K] bytes, sw [blocks of N][groups of K]; out [M,N] float or bfloat16.
-// flags: 1 the weights were written long before, they may be read while the kernel in front still runs.
-ACV_API int acv_gemm_fp8_rows(const void* x, long long ldx, const float* sx, long long ldsx, const void* w, long long ldw, const float* sw,
-                              long long ldsw, void* out, long long ldo, int out_f32, int M, int N, int K, int flags, int sms, cudaStream_t stream) {
-    if (M <= 0 || N <= 0) return 0;
-    if (K <= 0) return ACV_ERR_SIZE;
-    Fp8RowsParams p = {};
-    p.x = (const uint8_t*)x; p.w = (const uint8_t*)w; p.sx = sx; p.sw = sw; p.out = out;
-    p.ldx = ldx; p.ldw = ldw; p.ldo = ldo; p.ldsx = ldsx; p.ldsw = ldsw;
-    p.M = M; p.N = N; p.K = K; p.G = (K + FP8_GROUP - 1) / FP8_GROUP; p.out_f32 = out_f32; p.early_w = flags & 1;
-    if (const int e = fr_checks(p)) return e;
-    if (M > 8) return fr_launch<4, 2, 3>(p, sms, stream);
-    return fr_launch<4, 1, 3>(p, sms, stream);
-}
-
-// The same for gate and up rows [N,K] each: out [M,N] bytes = silu(gate) * up by its own scales so [M][groups of N].
-ACV_API int acv_gemm_fp8_rows_gated(const void* x, long long ldx, const float* sx, long long ldsx, const void* w, long long ldw, const float* sw,
-                                    long long ldsw, const void* w2, long long ldw2, const float* sw2, long long ldsw2, void* out,
-                                    long long ldo, float* so, long long ldso, int M, int N, int K, int flags, int sms, cudaStream_t stream) {
-    if (M <= 0 || N <= 0) return 0;
-    if (K <= 0) return ACV_ERR_SIZE;
-    Fp8RowsParams p = {};
-    p.x = (const uint8_t*)x; p.w = (const uint8_t*)w; p.w2 = (const uint8_t*)w2; p.sx = sx; p.sw = sw; p.sw2 = sw2; p.out = out; p.so = so;
-    p.ldx = ldx; p.ldw = ldw; p.ldw2 = ldw2; p.ldo = ldo; p.ldsx = ldsx; p.ldsw = ldsw; p.ldsw2 = ldsw2; p.ldso = ldso;
-    p.M = M; p.N = N; p.K = K; p.G = (K + FP8_GROUP - 1) / FP8_GROUP; p.early_w = flags & 1;
-    if (const int e = fr_checks(p)) return e;
-    if (M > 8) return fg_launch<2, 6>(p, stream);
-    return fg_launch<1, 6>(p, stream);
+    if (p.w2) return p.M > 8 ? fg_launch<2, 6>(p, stream) : fg_launch<1, 6>(p, stream);
+    return p.M > 8 ? fr_launch<4, 2, 3>(p, sms, stream) : fr_launch<4, 1, 3>(p, sms, stream);
 }

@@ -1,0 +1,729 @@
+// The products of e4m3 operands with block scales on the fifth-generation tensor cores.
+//
+//   y[t][n] = sum over groups g of 128 k of  sx[t][g] sw[n / 128][g] P_g[t][n],   P_g[t][n] = sum over k in g of qx[t][k] qw[n][k]
+//
+// P_g is what tcgen05.mma (kind::f8f6f4, operands staged by TMA, 128-byte swizzle: a k-block of 128 is one swizzle row) leaves in
+// tensor memory for one k-block.  It cannot stay there: its scales differ from k-block to k-block.  Tensor memory holds two such
+// partial tiles; while the tensor core fills one, eight epilogue warps fetch the other and add it, times its scales, to the float
+// sums that they hold in registers (a fused multiply-add for each output and k-block, two at a time as fma.rn.f32x2).  Tokens are
+// the rows (a lane holds one, so sx is a number of the thread's), features the columns (128 of them, one block row of sw, to a
+// thread or two).
+//
+// Two forms.  Pairs of CTAs on tiles of 256 x 256 (cta_group::2), persistent, for many tokens: a CTA loads 128 rows of each operand
+// for a k-block, 32 KB for 512 cycles of tensor core.  And single CTAs on tiles of 128 x BN, one each, for fewer: K may be split over
+// the CTAs of a cluster, whose sums meet through its shared memory, in rank order, so the result does not depend on timing.
+//
+// Warps: 0 loads, 1 issues the products, 2..9 are the epilogue, two to each quarter of the lanes.  Every wait on an mbarrier is
+// bounded; when one runs out the kernel records where in `status`, all roles leave their loops, the loads in flight are waited for
+// (with a limit), tensor memory is freed and the kernel returns.
+#include "fp8.cuh"
+#include "tc_ptx.cuh"
+#include "tensor_map.h"
+#include "gemm_fp8.h"
+
+#define FT_THREADS 320
+#define FT_ROWS 128                         // rows of an operand tile = bytes of a k-block's row
+#define FT_TILE (FT_ROWS * FT_ROWS)         // bytes of an operand tile of 128 rows
+
+struct Fp8TcParams {
+    int M, N, n_kb;                         // N: features, or units of the gated form
+    const float *sx, *sw, *sw2;             // sw2: the up rows' scales of the gated form
+    long long ldsx, ldsw, ldsw2, ldo, ldso;
+    void* out;
+    float* so;
+    int out_f32, out_vec;                   // out_vec: rows of out take 16-byte stores
+    int tiles_m, tiles_n, group, stages, splits, kb_per_split, early_w;
+    int* status;
+    unsigned int wait_limit;                // of polls; less and a k-block whose loads are left out (skip_kb >= 0) in the test of the waits only
+    int skip_kb;
+};
+
+__device__ __forceinline__ uint32_t ft_idesc(int n, int m) {        // float accumulator, e4m3 operands (type 0), both K-major
+    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <bool PAIR>
+__device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI) : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI) : "memory");
+}
+// the registers of a load are what its wait hands over: nothing that reads them moves in front of it
+__device__ __forceinline__ void ft_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+}
+__device__ __forceinline__ void ft_fma2(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t scale) {
+    asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(scale));
+}
+__device__ __forceinline__ uint64_t ft_both(float v) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(v)));
+    return r;
+}
+__device__ __forceinline__ float2 ft_floats(uint64_t v) {
+    uint32_t lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+
+// sums[0 .. 8 PIECES) += scale * the tile's 16 PIECES columns, a piece from `first` + 16 i (from `second` + 16 (i - PIECES / 2) in the
+// second half); the next piece is on its way while one is added
+template <int PIECES>
+__device__ __forceinline__ void ft_add_tile(uint64_t (&sums)[8 * PIECES], uint32_t first, uint32_t second, float scale1, float scale2) {
+    const uint64_t s1 = ft_both(scale1), s2 = ft_both(scale2);
+    uint32_t r[2][16];
+    tc_ld16_nowait(first, r[0]);
+    ft_wait_ld(r[0]);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        if (i + 1 < PIECES) tc_ld16_nowait(i + 1 < PIECES / 2 ? first + 16 * (i + 1) : second + 16 * (i + 1 - PIECES / 2), r[(i + 1) & 1]);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) ft_fma2(sums[8 * i + c], r[i & 1][2 * c], r[i & 1][2 * c + 1], i < PIECES / 2 ? s1 : s2);
+        if (i + 1 < PIECES) ft_wait_ld(r[(i + 1) & 1]);
+    }
+}
+
+// sixteen neighbouring outputs of a row
+__device__ __forceinline__ void ft_store16(const Fp8TcParams& p, int row, int n, const uint64_t* v) {
+    if (row >= p.M || n >= p.N) return;
+    float f[16];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const float2 t = ft_floats(v[c]);
+        f[2 * c] = t.x;
+        f[2 * c + 1] = t.y;
+    }
+    if (p.out_f32) {
+        float* o = reinterpret_cast<float*>(p.out) + (size_t)row * p.ldo + n;
+        if (p.out_vec && n + 16 <= p.N) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) reinterpret_cast<float4*>(o)[c] = make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+                if (n + c < p.N) o[c] = f[c];
+        }
+    } else {
+        bf16* o = reinterpret_cast<bf16*>(p.out) + (size_t)row * p.ldo + n;
+        if (p.out_vec && n + 16 <= p.N) {
+            uint32_t w[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) w[c] = pack_bf16x2(f[2 * c], f[2 * c + 1]);
+            reinterpret_cast<uint4*>(o)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4*>(o)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c)
+                if (n + c < p.N) o[c] = __float2bfloat16_rn(f[c]);
+        }
+    }
+}
+
+__device__ __forceinline__ void ft_tile_of(int tile, int tiles_m, int tiles_n, int group, int& ta, int& tb) {
+    const int per_group = group * tiles_n, g = tile / per_group, r = tile - g * per_group, rows = min(group, tiles_m - g * group);
+    tb = r / rows;
+    ta = g * group + (r - tb * rows);
+}
+// After a wait that ran out: the loads that are still under way write into this CTA's shared memory, so their stages are waited for
+// (each by the parity of the last of `asked` k-blocks that went into it), with a limit.
+__device__ __forceinline__ void ft_drain(uint32_t full0, int stages, int asked, unsigned int limit) {
+    for (int s = 0; s < stages && s < asked; ++s) {
+        const int last = (asked - 1 - s) / stages;
+        for (unsigned int i = 0; i < limit; ++i)
+            if (mbar_try_wait(full0 + 8 * s, last & 1)) break;
+    }
+}
+
+// the epilogue's wait, by a whole warp: true for all of its lanes where it ran out for one
+__device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Fp8TcParams& p) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit));
+    if (!ok && (threadIdx.x & 31) == 0) {
+        *abort_flag = 1;
+        atomicExch(p.status, 4);
+    }
+    return !ok;
+}
+
+// ----------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256
+#define FP_STAGE (2 * FT_TILE)              // a CTA's share of a k-block: 128 rows of tokens, 128 of weights
+#define FP_MAX_STAGES 6
+
+// GATED: the tile's columns are 128 units' gate rows (the leader's half of the weight tile) and the same units' up rows (the other's).
+template <bool GATED>
+__global__ void __launch_bounds__(FT_THREADS, 1)
+gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_w2, const Fp8TcParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = smem_raw + ((1024u - (gt_smem(smem_raw) & 1023u)) & 1023u);
+    const int STAGES = p.stages;
+    const uint32_t tiles_addr = gt_smem(tiles);
+    // barriers: full[STAGES] (the leader's count both CTAs' bytes), empty[STAGES], tmem_full[2], tmem_empty[2] (the leader's)
+    const uint32_t full0 = tiles_addr + STAGES * FP_STAGE, empty0 = full0 + 8 * STAGES, tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ volatile int abort_s;
+    __shared__ uint32_t most[GATED ? 2 : 1][2][FT_ROWS];
+    __shared__ __align__(8) uint64_t met[4];            // the two warps of a quarter of the lanes tell each other their maxima
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, n_items = p.tiles_m * p.tiles_n;
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 16); }
+        for (int q = 0; q < 4; ++q) mbar_init(gt_smem(&met[q]), 2);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gt_smem(&tmem_base_s)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();         // both CTAs' barriers exist before a load or a commit of the other arrives at them
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_s;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            const uint32_t lead_full0 = cluster_map(full0, 0);
+            const CUtensorMap* weights = GATED && rank == 1 ? &map_w2 : &map_w;
+            auto weight_row = [&](int tb) { return GATED ? tb * FT_ROWS : tb * 2 * FT_ROWS + (int)rank * FT_ROWS; };
+            int early = 0, asked = 0;
+            if (p.early_w && pair < n_items) {
+                int ta, tb;
+                ft_tile_of(pair, p.tiles_m, p.tiles_n, p.group, ta, tb);
+                early = min(STAGES, p.n_kb);
+                for (int i = 0; i < early; ++i) {
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * i, 2 * FP_STAGE);
+                    tma_load_2d_pair(tiles_addr + i * FP_STAGE + FT_TILE, weights, lead_full0 + 8 * i, i * FT_ROWS, weight_row(tb));
+                }
+            }
+            pdl_wait();
+            int s = 0;
+            uint32_t ph = 0;
+            for (int item = pair; item < n_items && !abort_s; item += n_pairs) {
+                int ta, tb;
+                ft_tile_of(item, p.tiles_m, p.tiles_n, p.group, ta, tb);
+                for (int kb = 0; kb < p.n_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                    const uint32_t dst = tiles_addr + s * FP_STAGE;
+                    const bool half_done = early > 0;
+                    if (half_done) {
+                        --early;
+                    } else {
+                        if (!mbar_wait(empty0 + 8 * s, ph ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 1); break; }
+                        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * FP_STAGE);
+                    }
+                    ++asked;
+                    if (kb == p.skip_kb) continue;
+                    tma_load_2d_pair(dst, &map_x, lead_full0 + 8 * s, kb * FT_ROWS, ta * 2 * FT_ROWS + (int)rank * FT_ROWS);
+                    if (!half_done) tma_load_2d_pair(dst + FT_TILE, weights, lead_full0 + 8 * s, kb * FT_ROWS, weight_row(tb));
+                }
+            }
+            if (abort_s && rank == 0) ft_drain(full0, STAGES, asked, p.wait_limit);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            pdl_wait();         // (the first tokens come after it: the wait for them starts there)
+            const uint32_t idesc = ft_idesc(2 * FT_ROWS, 2 * FT_ROWS);
+            const uint32_t a_lo0 = umma_desc_lo(tiles_addr), b_lo0 = umma_desc_lo(tiles_addr + FT_TILE);
+            uint32_t turn = 0, ph = 0, s_lo = 0;
+            int s = 0;
+            bool failed = false;
+            for (int item = pair; item < n_items && !abort_s && !failed; item += n_pairs) {
+                for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
+                    const uint32_t buf = turn & 1, use = turn >> 1;
+                    if (!mbar_wait(full0 + 8 * s, ph, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 3); failed = true; break; }
+                    if (!mbar_wait(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 2); failed = true; break; }
+                    tc_fence_after();
+                    const uint32_t d = tmem_base + buf * 2 * FT_ROWS, a_lo = a_lo0 + s_lo, b_lo = b_lo0 + s_lo;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) ft_mma<true>(d, a_lo + 2 * k, b_lo + 2 * k, idesc, k > 0);
+                    tc_commit_pair(empty0 + 8 * s, 3);
+                    tc_commit_pair(tfull0 + 8 * buf, 3);
+                    ++s; s_lo += FP_STAGE >> 4;
+                    if (s == STAGES) { s = 0; s_lo = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else {
+        const int wq = warp & 3, half = (warp - 2) >> 2;
+        pdl_wait();
+        const uint32_t lead_tempty0 = cluster_map(tempty0, 0);
+        const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16);
+        uint32_t turn = 0, parity = 0;
+        // (a warp gives up as a whole: its loads from tensor memory and its exchanges are the whole warp's)
+        bool failed = false;
+        for (int item = pair; item < n_items && !failed; item += n_pairs) {
+            int ta, tb;
+            ft_tile_of(item, p.tiles_m, p.tiles_n, p.group, ta, tb);
+            const int row = ta * 2 * FT_ROWS + (int)rank * FT_ROWS + wq * 32 + lane;
+            // (rows and blocks that do not exist have products of zeros: any scale that does exist will do)
+            const float* sx = p.sx + (size_t)min(row, p.M - 1) * p.ldsx;
+            const int block = GATED ? tb : min(tb * 2 + half, (p.N - 1) / FT_ROWS);
+            const float *sw = p.sw + (size_t)block * p.ldsw, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : nullptr;
+            uint64_t sums[64];
+#pragma unroll
+            for (int i = 0; i < 64; ++i) sums[i] = 0;
+            float next_x = __ldg(sx), next_w = __ldg(sw), next_w2 = GATED ? __ldg(sw2) : 0.f;
+            for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
+                const float a = next_x, b = next_w, b2 = next_w2;
+                if (kb + 1 < p.n_kb) {
+                    next_x = __ldg(sx + kb + 1);
+                    next_w = __ldg(sw + kb + 1);
+                    if (GATED) next_w2 = __ldg(sw2 + kb + 1);
+                }
+                const uint32_t buf = turn & 1, use = turn >> 1;
+                failed = ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p);
+                if (failed) break;
+                tc_fence_after();
+                const uint32_t t = taddr + buf * 2 * FT_ROWS;
+                if (GATED) ft_add_tile<8>(sums, t + half * 64, t + FT_ROWS + half * 64, a * b, a * b2);
+                else ft_add_tile<8>(sums, t + half * FT_ROWS, t + half * FT_ROWS + 64, a * b, a * b);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (rank == 0) mbar_arrive(tempty0 + 8 * buf);
+                    else mbar_arrive_remote(lead_tempty0 + 8 * buf);
+                }
+            }
+            if (failed) break;
+            if (!GATED) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ft_store16(p, row, tb * 2 * FT_ROWS + half * FT_ROWS + 16 * i, sums + 8 * i);
+            } else {
+                // silu(gate) * up of 64 units; the other 64 of the group are the partner warp's
+                uint32_t m = 0;
+                float act[64];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float2 g = ft_floats(sums[i]), u = ft_floats(sums[32 + i]);
+                    act[2 * i] = silu_f32<float>(g.x) * u.x;
+                    act[2 * i + 1] = silu_f32<float>(g.y) * u.y;
+                    m = max(m, max(fp8_magnitude(act[2 * i]), fp8_magnitude(act[2 * i + 1])));
+                }
+                most[parity][half][wq * 32 + lane] = m;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(gt_smem(&met[wq]));
+                failed = ft_warp_failed(gt_smem(&met[wq]), parity, &abort_s, p);
+                if (failed) break;
+                const Fp8Scale k = fp8_scale(max(m, most[parity][half ^ 1][wq * 32 + lane]));
+                parity ^= 1;
+                const int u0 = tb * FT_ROWS + half * 64;
+                if (row < p.M) {
+                    if (half == 0) p.so[(size_t)row * p.ldso + tb] = k.s;
+                    uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + (size_t)row * p.ldo + u0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) w[c] = fp8_pack4(act[16 * i + 4 * c], act[16 * i + 4 * c + 1], act[16 * i + 4 * c + 2], act[16 * i + 4 * c + 3], k.r);
+                        if (p.out_vec && u0 + 16 * i + 16 <= p.N) {
+                            *reinterpret_cast<uint4*>(o + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 16; ++c)
+                                if (u0 + 16 * i + c < p.N) o[16 * i + c] = (uint8_t)(w[c >> 2] >> (8 * (c & 3)));
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // neither CTA leaves, nor is the pair's tensor memory given back, while the other may still use this one's
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
+    }
+}
+
+// ----------------------------------------------------------------------------- single CTAs, tiles of 128 x BN, K over a cluster
+template <int BN>
+struct Fp8TileShape {
+    static constexpr int STAGE = FT_TILE + BN * FT_ROWS;
+    static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int LD = BN + 4;                               // floats of a row of the summed tile: sixteen-byte stores of eight rows meet no bank twice
+    static constexpr int SUMS = FT_ROWS * LD * 4;
+    static constexpr int smem(int stages) { return 1024 + (stages * STAGE > SUMS ? stages * STAGE : SUMS) + 256; }
+};
+
+__device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// GATED: BN is 256, the columns are 128 units' gate rows and their up rows, and a row of the result is a whole group.
+template <int BN, bool GATED>
+__global__ void __launch_bounds__(FT_THREADS, 1)
+gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_w2, const Fp8TcParams p) {
+    using S = Fp8TileShape<BN>;
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* tiles = smem_raw + ((1024u - (gt_smem(smem_raw) & 1023u)) & 1023u);
+    const int STAGES = p.stages;
+    const uint32_t tiles_addr = gt_smem(tiles);
+    const uint32_t full0 = tiles_addr + (STAGES * S::STAGE > S::SUMS ? STAGES * S::STAGE : S::SUMS), empty0 = full0 + 8 * STAGES;
+    const uint32_t tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ volatile int abort_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, ta = tile % p.tiles_m, tb = tile / p.tiles_m;
+    const int kb0 = split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.n_kb);
+    if (threadIdx.x == 0) {
+        abort_s = 0;
+        for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+        for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 8); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(gt_smem(&tmem_base_s)), "r"(S::TMEM));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = tmem_base_s;
+    pdl_launch_dependents();
+    const int row_here = ta * FT_ROWS;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            auto load_w = [&](int s, int kb) {
+                const uint32_t dst = tiles_addr + s * S::STAGE + FT_TILE;
+                if (GATED) {
+                    tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS);
+                    tma_load_2d(dst + FT_TILE, &map_w2, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS);
+                } else {
+                    tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * BN);
+                }
+            };
+            const int early = p.early_w ? min(STAGES, kb1 - kb0) : 0;
+            for (int i = 0; i < early; ++i) {
+                mbar_expect_tx(full0 + 8 * i, S::STAGE);
+                load_w(i, kb0 + i);
+            }
+            pdl_wait();
+            int s = 0, asked = 0;
+            uint32_t ph = 0;
+            for (int kb = kb0; kb < kb1; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
+                const bool half_done = kb - kb0 < early;
+                if (!half_done) {
+                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 1); break; }
+                    mbar_expect_tx(full0 + 8 * s, S::STAGE);
+                }
+                ++asked;
+                if (kb == p.skip_kb) continue;
+                tma_load_2d(tiles_addr + s * S::STAGE, &map_x, full0 + 8 * s, kb * FT_ROWS, row_here);
+                if (!half_done) load_w(s, kb);
+            }
+            if (abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            pdl_wait();
+            const uint32_t idesc = ft_idesc(BN, FT_ROWS);
+            const uint32_t a_lo0 = umma_desc_lo(tiles_addr), b_lo0 = umma_desc_lo(tiles_addr + FT_TILE);
+            uint32_t turn = 0, ph = 0, s_lo = 0;
+            int s = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++turn) {
+                const uint32_t buf = turn & 1, use = turn >> 1;
+                if (!mbar_wait(full0 + 8 * s, ph, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 3); break; }
+                if (!mbar_wait(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 2); break; }
+                tc_fence_after();
+                const uint32_t d = tmem_base + buf * BN, a_lo = a_lo0 + s_lo, b_lo = b_lo0 + s_lo;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ft_mma<false>(d, a_lo + 2 * k, b_lo + 2 * k, idesc, k > 0);
+                tc_commit(empty0 + 8 * s);
+                tc_commit(tfull0 + 8 * buf);
+                ++s; s_lo += S::STAGE >> 4;
+                if (s == STAGES) { s = 0; s_lo = 0; ph ^= 1; }
+            }
+        }
+    } else {
+        constexpr int PIECES = BN / 32;             // of sixteen columns: a thread's half of the tile
+        const int wq = warp & 3, half = (warp - 2) >> 2;
+        pdl_wait();
+        const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16);
+        const int r = wq * 32 + lane;
+        const float* sx = p.sx + (size_t)min(row_here + r, p.M - 1) * p.ldsx;
+        const int block = GATED ? tb : min((tb * BN + (BN > FT_ROWS ? half * FT_ROWS : 0)) / FT_ROWS, (p.N - 1) / FT_ROWS);
+        const float *sw = p.sw + (size_t)block * p.ldsw, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : nullptr;
+        uint64_t sums[8 * PIECES];
+#pragma unroll
+        for (int i = 0; i < 8 * PIECES; ++i) sums[i] = 0;
+        float next_x = __ldg(sx + kb0), next_w = __ldg(sw + kb0), next_w2 = GATED ? __ldg(sw2 + kb0) : 0.f;
+        uint32_t turn = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++turn) {
+            const float a = next_x, b = next_w, b2 = next_w2;
+            if (kb + 1 < kb1) {
+                next_x = __ldg(sx + kb + 1);
+                next_w = __ldg(sw + kb + 1);
+                if (GATED) next_w2 = __ldg(sw2 + kb + 1);
+            }
+            const uint32_t buf = turn & 1, use = turn >> 1;
+            if (ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p)) break;
+            tc_fence_after();
+            const uint32_t t = taddr + buf * BN;
+            if (GATED) ft_add_tile<PIECES>(sums, t + half * 64, t + FT_ROWS + half * 64, a * b, a * b2);
+            else ft_add_tile<PIECES>(sums, t + half * (BN / 2), t + half * (BN / 2) + BN / 4, a * b, a * b);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(tempty0 + 8 * buf);
+        }
+        // Every load has landed and every product has read it: the stages' place takes the tile's sums, [row][column].  (After a wait
+        // that ran out neither is sure, and nothing is written.)
+        if (!abort_s && row_here + r < p.M) {
+            float* to = reinterpret_cast<float*>(tiles) + r * S::LD;
+#pragma unroll
+            for (int i = 0; i < 4 * PIECES; ++i) {
+                const float2 lo = ft_floats(sums[2 * i]), hi = ft_floats(sums[2 * i + 1]);
+                const int c = GATED ? (i < 2 * PIECES ? half * 64 + 4 * i : FT_ROWS + half * 64 + 4 * (i - 2 * PIECES)) : half * (BN / 2) + 4 * i;
+                *reinterpret_cast<float4*>(to + c) = make_float4(lo.x, lo.y, hi.x, hi.y);
+            }
+        }
+    }
+    tc_fence_before();
+    if (p.splits > 1) cluster_sync_all();
+    else __syncthreads();
+    // The rows of the tile are dealt out to the cluster's CTAs and their warps; a lane takes four neighbouring columns at a time.
+    const int rows = min(FT_ROWS, p.M - row_here);
+    const uint32_t own = tiles_addr;
+    if (!abort_s) {
+#pragma unroll 1
+        for (int r = split + p.splits * warp; r < rows; r += p.splits * (FT_THREADS / 32)) {
+            auto sum4 = [&](int c) {
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                const uint32_t at = own + (uint32_t)(r * S::LD + c) * 4;
+                for (int q = 0; q < p.splits; ++q) {
+                    const float4 o = ft_cluster_read4(cluster_map(at, q));
+                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
+                }
+                return v;
+            };
+            const size_t row = (size_t)(row_here + r);
+            if (GATED) {
+                const float4 g = sum4(4 * lane), u = sum4(FT_ROWS + 4 * lane);
+                const float h[4] = {silu_f32<float>(g.x) * u.x, silu_f32<float>(g.y) * u.y, silu_f32<float>(g.z) * u.z, silu_f32<float>(g.w) * u.w};
+                uint32_t m = max(max(fp8_magnitude(h[0]), fp8_magnitude(h[1])), max(fp8_magnitude(h[2]), fp8_magnitude(h[3])));
+                m = __reduce_max_sync(0xffffffffu, m);
+                const Fp8Scale k = fp8_scale(m);
+                const uint32_t w = fp8_pack4(h[0], h[1], h[2], h[3], k.r);
+                if (lane == 0) p.so[row * p.ldso + tb] = k.s;
+                const int u0 = tb * FT_ROWS + 4 * lane;
+                uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + row * p.ldo + u0;
+                if (p.out_vec && u0 + 4 <= p.N) {
+                    *reinterpret_cast<uint32_t*>(o) = w;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (u0 + c < p.N) o[c] = (uint8_t)(w >> (8 * c));
+                }
+            } else {
+#pragma unroll
+                for (int c = 4 * lane; c < BN; c += 128) {
+                    const float4 v = sum4(c);
+                    const int n = tb * BN + c;
+                    if (n >= p.N) continue;
+                    if (p.out_f32) {
+                        float* o = reinterpret_cast<float*>(p.out) + row * p.ldo + n;
+                        if (p.out_vec && n + 4 <= p.N) {
+                            *reinterpret_cast<float4*>(o) = v;
+                        } else {
+                            o[0] = v.x;
+                            if (n + 1 < p.N) o[1] = v.y;
+                            if (n + 2 < p.N) o[2] = v.z;
+                            if (n + 3 < p.N) o[3] = v.w;
+                        }
+                    } else {
+                        bf16* o = reinterpret_cast<bf16*>(p.out) + row * p.ldo + n;
+                        if (p.out_vec && n + 4 <= p.N) {
+                            *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
+                        } else {
+                            o[0] = __float2bfloat16_rn(v.x);
+                            if (n + 1 < p.N) o[1] = __float2bfloat16_rn(v.y);
+                            if (n + 2 < p.N) o[2] = __float2bfloat16_rn(v.z);
+                            if (n + 3 < p.N) o[3] = __float2bfloat16_rn(v.w);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // (the peers may still read this CTA's sums)
+    if (p.splits > 1) cluster_sync_all();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
+    }
+}
+
+// ----------------------------------------------------------------------------- host side
+// tensor map of a matrix of bytes [rows, K] with row stride ld: box = 128 x box_rows, 128-byte swizzle
+static int ft_map(CUtensorMap* map, const void* base, int rows, int K, long long ld, int box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return ACV_ERR_SIZE;
+    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {FT_ROWS, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : ACV_ERR_ALIGN;
+}
+
+// Test of the bounded waits, without a fault: the next product launched from this process polls each mbarrier at most `wait_limit`
+// times and its producer leaves out the loads of k-block `skip_kb` (the codes are those of acv_gemm_tc_test_fault; the output of that
+// launch is unspecified).
+static unsigned int g_test_wait_limit = 0;
+static int g_test_skip_kb = -1;
+ACV_API void acv_gemm_fp8_test_fault(int wait_limit, int skip_kb) {
+    g_test_wait_limit = wait_limit > 0 ? (unsigned int)wait_limit : 0u;
+    g_test_skip_kb = skip_kb;
+}
+
+template <bool GATED>
+static int ft_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mw2, Fp8TcParams& p, int sms, cudaStream_t stream) {
+    p.stages = FP_MAX_STAGES;
+    const int smem = FP_MAX_STAGES * FP_STAGE + 1024 + 256;
+    auto kernel = gemm_fp8_pair_kernel<GATED>;
+    static AcvSmemConfig cfg;
+    if (const int rc = acv_ensure_smem(cfg, kernel, smem)) return rc;
+    // pairs that can be resident at once: two free SMs side by side each, which an odd number of SMs in a part of the chip does not give
+    static std::mutex mu;
+    static int pairs_of_device[64];
+    int dev = 0, resident = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return ACV_ERR_SIZE;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        resident = pairs_of_device[dev];
+        if (resident <= 0) {
+            cudaLaunchConfig_t lc = {};
+            lc.gridDim = dim3(2 * (sms / 2));
+            lc.blockDim = dim3(FT_THREADS);
+            lc.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+            lc.attrs = attr;
+            lc.numAttrs = 1;
+            if (cudaOccupancyMaxActiveClusters(&resident, kernel, &lc) != cudaSuccess || resident <= 0) {
+                cudaGetLastError();
+                return ACV_ERR_SIZE;
+            }
+            pairs_of_device[dev] = resident;
+        }
+    }
+    p.tiles_m = (p.M + 2 * FT_ROWS - 1) / (2 * FT_ROWS);
+    p.tiles_n = (p.N + (GATED ? 1 : 2) * FT_ROWS - 1) / ((GATED ? 1 : 2) * FT_ROWS);
+    p.group = 8;
+    const long long items = (long long)p.tiles_m * p.tiles_n;
+    if (items > 0x7fffffff) return ACV_ERR_SIZE;
+    const int pairs = (int)(items < resident ? items : resident);
+    acv_launch_cluster(PDL_GEMM, dim3(2, 1, 1), kernel, dim3(2 * pairs), dim3(FT_THREADS), smem, stream, mx, mw, mw2, p);
+    return acv_launch_status();
+}
+
+template <int BN, bool GATED>
+static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mw2, Fp8TcParams& p, int splits, cudaStream_t stream) {
+    using S = Fp8TileShape<BN>;
+    p.tiles_m = (p.M + FT_ROWS - 1) / FT_ROWS;
+    p.tiles_n = (p.N + (GATED ? FT_ROWS : BN) - 1) / (GATED ? FT_ROWS : BN);
+    if (splits < 1) splits = 1;
+    if (splits > 8) splits = 8;
+    if (splits > p.n_kb) splits = p.n_kb;
+    p.kb_per_split = (p.n_kb + splits - 1) / splits;
+    p.splits = (p.n_kb + p.kb_per_split - 1) / p.kb_per_split;
+    p.stages = min(8, 200 * 1024 / S::STAGE);
+    const int smem = S::smem(p.stages);
+    auto kernel = gemm_fp8_tile_kernel<BN, GATED>;
+    static AcvSmemConfig cfg;
+    if (const int rc = acv_ensure_smem(cfg, kernel, smem)) return rc;
+    const long long ctas = (long long)p.tiles_m * p.tiles_n * p.splits;
+    if (ctas > 0x7fffffff) return ACV_ERR_SIZE;
+    acv_launch_cluster(PDL_GEMM, dim3(p.splits, 1, 1), kernel, dim3((unsigned)ctas), dim3(FT_THREADS), smem, stream, mx, mw, mw2, p);
+    return acv_launch_status();
+}
+
+// How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs.
+struct Fp8Plan { int kind, bn, splits; };
+static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
+    if (M <= 16) return {1, 0, 1};
+    const int n_kb = (K + FT_ROWS - 1) / FT_ROWS, tm = (M + FT_ROWS - 1) / FT_ROWS;
+    const int bn = gated ? 256 : 128, tiles = tm * ((N + FT_ROWS - 1) / FT_ROWS);
+    if (tiles > sms) return {3, 256, 1};
+    int splits = 1;
+    while (splits < 8 && splits < n_kb && tiles <= ACV_CLUSTERS_AT_ONCE[splits + 1]) ++splits;
+    return {2, bn, splits};
+}
+
+static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cudaStream_t stream) {
+    const bool gated = o.w2 != nullptr;
+    if (o.M <= 0 || o.N <= 0) return 0;
+    if (o.K <= 0) return ACV_ERR_SIZE;
+    if (((uintptr_t)o.x | (uintptr_t)o.w | (uintptr_t)o.w2) % 16 || (o.ldx | o.ldw | o.ldw2) % 16) return ACV_ERR_ALIGN;
+    const Fp8Plan how = plan ? Fp8Plan{plan & 15, (plan >> 4) & 0xfff, plan >> 16} : ft_plan(o.M, o.N, o.K, gated, sms);
+    if (how.kind == 1) return acv_fp8_rows(o, flags, sms, stream);
+    if (!status) return ACV_ERR_SCRATCH;
+    Fp8TcParams p = {};
+    p.M = o.M; p.N = o.N; p.n_kb = (o.K + FT_ROWS - 1) / FT_ROWS;
+    p.sx = o.sx; p.sw = o.sw; p.sw2 = o.sw2; p.ldsx = o.ldsx; p.ldsw = o.ldsw; p.ldsw2 = o.ldsw2; p.ldo = o.ldo; p.ldso = o.ldso;
+    p.out = o.out; p.so = o.so; p.out_f32 = o.out_f32; p.early_w = flags & 1; p.status = status;
+    p.out_vec = fp8_rows_aligned(o.out, o.ldo, gated ? 1 : o.out_f32 ? 4 : 2, 16);
+    p.wait_limit = g_test_wait_limit ? g_test_wait_limit : GT_WAIT_LIMIT;
+    p.skip_kb = g_test_skip_kb;
+    g_test_wait_limit = 0; g_test_skip_kb = -1;
+    CUtensorMap mx, mw, mw2;
+    if (const int rc = ft_map(&mx, o.x, o.M, o.K, o.ldx, FT_ROWS)) return rc;
+    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 3 || gated ? FT_ROWS : how.bn)) return rc;
+    mw2 = mw;
+    if (gated)
+        if (const int rc = ft_map(&mw2, o.w2, o.N, o.K, o.ldw2, FT_ROWS)) return rc;
+    if (how.kind == 3) return gated ? ft_launch_pair<true>(mx, mw, mw2, p, sms, stream) : ft_launch_pair<false>(mx, mw, mw2, p, sms, stream);
+    if (how.kind != 2) return ACV_ERR_SIZE;
+    if (gated) return how.bn == 256 ? ft_launch_tile<256, true>(mx, mw, mw2, p, how.splits, stream) : ACV_ERR_SIZE;
+    switch (how.bn) {
+        case 64: return ft_launch_tile<64, false>(mx, mw, mw2, p, how.splits, stream);
+        case 128: return ft_launch_tile<128, false>(mx, mw, mw2, p, how.splits, stream);
+        default: return ACV_ERR_SIZE;
+    }
+}
+
+// x [M,K] bytes, sx [M][groups of K]; w [N,K] bytes, sw [blocks of N][groups of K]; out [M,N] float or bfloat16; every matrix's rows at a
+// stride of its own, those of x and w on 16 bytes.  flags: 1 the weights were written long before, they may be read while the kernel
+// in front still runs.  plan: 0, or kind | bn << 4 | splits << 16.  status: one int, 0 unless a bounded wait ran out.
+ACV_API int acv_linear_fp8(const void* x, long long ldx, const float* sx, long long ldsx, const void* w, long long ldw, const float* sw,
+                           long long ldsw, void* out, long long ldo, int out_f32, int M, int N, int K, int flags, int plan, int* status,
+                           int sms, cudaStream_t stream) {
+    Fp8Operands o = {};
+    o.x = (const uint8_t*)x; o.w = (const uint8_t*)w; o.sx = sx; o.sw = sw; o.out = out;
+    o.ldx = ldx; o.ldw = ldw; o.ldo = ldo; o.ldsx = ldsx; o.ldsw = ldsw; o.M = M; o.N = N; o.K = K; o.out_f32 = out_f32;
+    return ft_run(o, flags, plan, status, sms, stream);
+}
+
+// The same for gate rows w and up rows w2 [N,K] each: out [M,N] bytes = silu(gate) * up by its own scales so [M][groups of N].
+ACV_API int acv_linear_fp8_swiglu(const void* x, long long ldx, const float* sx, long long ldsx, const void* w, long long ldw, const float* sw,
+                                  long long ldsw, const void* w2, long long ldw2, const float* sw2, long long ldsw2, void* out,
+                                  long long ldo, float* so, long long ldso, int M, int N, int K, int flags, int plan, int* status, int sms,
+                                  cudaStream_t stream) {
+    if (!w2) return ACV_ERR_SIZE;
+    Fp8Operands o = {};
+    o.x = (const uint8_t*)x; o.w = (const uint8_t*)w; o.w2 = (const uint8_t*)w2; o.sx = sx; o.sw = sw; o.sw2 = sw2; o.out = out; o.so = so;
+    o.ldx = ldx; o.ldw = ldw; o.ldw2 = ldw2; o.ldo = ldo; o.ldsx = ldsx; o.ldsw = ldsw; o.ldsw2 = ldsw2; o.ldso = ldso;
+    o.M = M; o.N = N; o.K = K;
+    return ft_run(o, flags, plan, status, sms, stream);
+}

@@ -148,8 +148,8 @@ def _declare(lib: ctypes.CDLL) -> None:
         "acv_gemm_tc_glu": [P, I, P, I, P, I, I, I, I, F, F, I, P, I, I, I, P],
         "acv_quantize_fp8": [P, I, LL, P, LL, P, LL, I, I, I, I, P],
         "acv_add_gated_norms": [P, I, LL, P, I, LL, P, I, LL, P, P, F, F, P, F, P, I, LL, P, LL, I, I, P],
-        "acv_gemm_fp8_rows": [P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, I, P],
-        "acv_gemm_fp8_rows_gated": [P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, P],
+        "acv_linear_fp8": [P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, I, P, I, P],
+        "acv_linear_fp8_swiglu": [P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, P, I, P],
         "acv_argmax": [P, I, I, I, P, P],
         "acv_apply_penalties": [P, I, I, P, P, P, I, P, P, P, P],
         "acv_sample": [P, I, I, I, P, P, P, P, P, P, P, P, P],
@@ -173,6 +173,8 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.acv_random_int.restype = c_int
     lib.acv_gemm_tc_test_fault.argtypes = [c_int, c_int]
     lib.acv_gemm_tc_test_fault.restype = None
+    lib.acv_gemm_fp8_test_fault.argtypes = [c_int, c_int]
+    lib.acv_gemm_fp8_test_fault.restype = None
 
 
 class DecodeLayerArgs(ctypes.Structure):
@@ -752,6 +754,11 @@ def gemm_tc_test_fault(wait_limit: int, skip_k_block: int) -> None:
     ``wait_limit`` times and never loads k-block ``skip_k_block``, so it gives up, frees what it holds, returns,
     and leaves the wait's code in the status word.  Nothing faults, traps or hangs."""
     library().acv_gemm_tc_test_fault(int(wait_limit), int(skip_k_block))
+
+
+def gemm_fp8_test_fault(wait_limit: int, skip_k_block: int) -> None:
+    """The same for the next 8-bit product on the tensor cores of this process."""
+    library().acv_gemm_fp8_test_fault(int(wait_limit), int(skip_k_block))
 
 
 def gemm_status(device=None) -> int:
@@ -2431,10 +2438,18 @@ def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, bl
     return values, scales
 
 
-def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+def _fp8_plan(plan: tuple | None) -> int:
+    return 0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16
+
+
+def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
+               plan: tuple | None = None) -> torch.Tensor:
     """out[T, N] = x @ w^T of quantised matrices: x [T, K] with a scale for each group of 128 of a row, w [N, K] with a scale for each
     block of 128 x 128; out float32 or bfloat16, dense rows at any stride.  A group's sum is multiplied by its two scales in float
-    and joins a float sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``)."""
+    and joins a float sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``).
+
+    The weights are read while the kernel in front of this one may still run: they were written long before.  ``plan``: (kind, columns
+    of a tile, splits of K) as csrc/gemm_fp8_tc.cu names them, in place of its own choice."""
     T, K = x.shape
     N = w.shape[0]
     _fp8_pair("linear_fp8", "x", x, x_scales, T, K, 1)
@@ -2446,14 +2461,15 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         return out
     if not K:
         return out.zero_()
-    _launch_on(device, "linear_fp8", library().acv_gemm_fp8_rows, x.data_ptr(), x.stride(0), x_scales.data_ptr(), x_scales.stride(0),
+    _launch_on(device, "linear_fp8", library().acv_linear_fp8, x.data_ptr(), x.stride(0), x_scales.data_ptr(), x_scales.stride(0),
                w.data_ptr(), w.stride(0), w_scales.data_ptr(), w_scales.stride(0), out.data_ptr(), out.stride(0),
-               1 if dtype_code(out.dtype) == F32 else 0, T, N, K, 1, sm_count(x.device))
+               1 if dtype_code(out.dtype) == F32 else 0, T, N, K, 1, _fp8_plan(plan), _status_pointer(x), sm_count(x.device))
     return out
 
 
 def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor,
-                      up_scales: torch.Tensor, out: torch.Tensor, out_scales: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+                      up_scales: torch.Tensor, out: torch.Tensor, out_scales: torch.Tensor,
+                      plan: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(out, out_scales) = silu(x @ gate^T) * (x @ up^T), quantised in groups of 128 units: what the next ``linear_fp8`` reads.
     Operands as there, gate and up [I, K] each with its own scales.  Unit and quantisation are float, from the float sums."""
     T, K = x.shape
@@ -2467,10 +2483,10 @@ def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tenso
         return out, out_scales
     if not K:
         raise KernelError("linear_fp8_swiglu: K is 0")
-    _launch_on(device, "linear_fp8_swiglu", library().acv_gemm_fp8_rows_gated, x.data_ptr(), x.stride(0), x_scales.data_ptr(),
+    _launch_on(device, "linear_fp8_swiglu", library().acv_linear_fp8_swiglu, x.data_ptr(), x.stride(0), x_scales.data_ptr(),
                x_scales.stride(0), gate.data_ptr(), gate.stride(0), gate_scales.data_ptr(), gate_scales.stride(0), up.data_ptr(),
                up.stride(0), up_scales.data_ptr(), up_scales.stride(0), out.data_ptr(), out.stride(0), out_scales.data_ptr(),
-               out_scales.stride(0), T, I, K, 1, sm_count(x.device))
+               out_scales.stride(0), T, I, K, 1, _fp8_plan(plan), _status_pointer(x), sm_count(x.device))
     return out, out_scales
 
 

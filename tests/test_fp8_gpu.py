@@ -105,12 +105,12 @@ def test_quantize_of_values_at_the_edges(block_rows, dtype):
 
 
 # ----------------------------------------------------------------------------- the product
-def check_product(T, N, K, out_dtype, seed, pads=(0, 0, 0)):
+def check_product(T, N, K, out_dtype, seed, pads=(0, 0, 0), plan=None):
     x, xs = quantized(T, K, seed, 1, pad=16 * pads[0])
     w, ws = quantized(N, K, seed + 1, 128, 0.02, pad=16 * pads[1])
     buf = torch.full((T + 1, N + 1 + pads[2]), 7.0, dtype=out_dtype, device=DEV)
     out = buf[:T, :N]
-    assert ops().linear_fp8(x, xs, w, ws, out) is out
+    assert ops().linear_fp8(x, xs, w, ws, out, plan=plan) is out
     want, error = pf.product(x, xs, w, ws)
     if out_dtype != F32:
         error = error + pf.half_step(want.abs() + error, out_dtype)
@@ -134,6 +134,18 @@ def test_product_of_other_sizes(T, N, K):
     check_product(T, N, K, F32, T + N + K, (1, 2, 3))
 
 
+@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 64, 1), (2, 64, 3), (2, 128, 1), (2, 128, 2), (2, 128, 8), (3, 256, 1)])
+@pytest.mark.parametrize("T,N,K,out_dtype", [(1, 128, 128, F32), (5, 300, 400, BF), (140, 130, 1100, F32), (300, 700, 2048, BF), (513, 257, 1296, F32)])
+def test_product_by_every_plan(T, N, K, out_dtype, plan):
+    check_product(T, N, K, out_dtype, T + 3, plan=plan)
+
+
+def test_products_of_many_tiles():
+    """More tiles than multiprocessors, so that a pair of CTAs walks several."""
+    check_product(1500, 6000, 272, BF, 5, plan=(3, 256, 1))
+    check_gated(1500, 4000, 272, 5, plan=(3, 256, 1))
+
+
 @pytest.mark.parametrize("T", [1, 12, 90, 400])
 def test_product_of_values_that_are_no_numbers(T):
     """A NaN or an infinity in a token's group, or an infinite scale, reaches that token's outputs and no other's."""
@@ -155,7 +167,7 @@ def test_product_of_values_that_are_no_numbers(T):
 
 
 # ----------------------------------------------------------------------------- the product with the gated unit
-def check_gated(T, I, K, seed, gate_factor=0.05):
+def check_gated(T, I, K, seed, gate_factor=0.05, plan=None):
     x, xs = quantized(T, K, seed, 1)
     g, gs = quantized(I, K, seed + 1, 128, gate_factor)
     u, us = quantized(I, K, seed + 2, 128, 0.02)
@@ -163,7 +175,7 @@ def check_gated(T, I, K, seed, gate_factor=0.05):
     out = buf.view(FP8)[:T, :I]
     sbuf = torch.full((T + 1, groups(I) + 1), 3.0, device=DEV)
     scales = sbuf[:T, :groups(I)]
-    ops().linear_fp8_swiglu(x, xs, g, gs, u, us, out, scales)
+    ops().linear_fp8_swiglu(x, xs, g, gs, u, us, out, scales, plan=plan)
     yg, eg = pf.product(x, xs, g, gs)
     yu, eu = pf.product(x, xs, u, us)
     h = yg * torch.sigmoid(yg) * yu
@@ -189,6 +201,38 @@ def test_gated_product(T, I, K):
 @pytest.mark.parametrize("T,I,K", [(1, 4096, 4096), (4, 300, 12288), (70, 130, 5120), (520, 2049, 272), (1030, 384, 640)])
 def test_gated_product_of_other_sizes(T, I, K):
     check_gated(T, I, K, T + I + K)
+
+
+@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 256, 1), (2, 256, 2), (2, 256, 5), (3, 256, 1)])
+@pytest.mark.parametrize("T,I,K", [(1, 128, 128), (5, 300, 400), (140, 130, 1100), (300, 700, 2048), (513, 257, 1296)])
+def test_gated_product_by_every_plan(T, I, K, plan):
+    check_gated(T, I, K, T + 3, plan=plan)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("kind", [2, 3])
+def test_a_wait_that_runs_out_is_reported(kind, gated):
+    """A product whose producer leaves out a k-block gives up after a few polls, says so in the status word, and the next one runs."""
+    x, xs = quantized(200, 1024, 1, 1)
+    w, ws = quantized(300, 1024, 2, 128)
+    plan = (kind, 256 if gated or kind == 3 else 128, 1)
+
+    def run():
+        if gated:
+            q, s = ops().fp8_rows(200, 300, DEV)
+            ops().linear_fp8_swiglu(x, xs, w, ws, w, ws, q, s, plan=plan)
+            return q.float()
+        return ops().linear_fp8(x, xs, w, ws, torch.empty((200, 300), device=DEV), plan=plan)
+
+    before = run()
+    assert ops().gemm_status() == 0
+    ops().gemm_fp8_test_fault(2000, 3)
+    run()
+    torch.cuda.synchronize()
+    assert ops().gemm_status() in (1, 2, 3, 4)
+    ops().reset_after_failure()
+    assert ops().gemm_status() == 0
+    assert torch.equal(run(), before) and ops().gemm_status() == 0
 
 
 # ----------------------------------------------------------------------------- the norms
