@@ -164,22 +164,32 @@ static int gn_launch(const GnParams& p, int T, cudaStream_t stream) {
     return acv_launch_status();
 }
 
-// x [T,H] in place; d [T,H] or null; gate: g [T,H] or gc float [H] or neither; w1 or null; out [T,H] of out_dtype (0 float, 1
-// bfloat16, 2 e4m3 with scales s [T][groups of H]) or null; every matrix's rows dense at a stride of its own.
-ACV_API int acv_add_gated_norms(void* x, int x_dtype, long long ldx, const void* d, int d_dtype, long long ldd, const void* g, int g_dtype,
-                                long long ldg, const float* gc, const float* w1, float e1, float c, const float* w2, float e2, void* out,
-                                int out_dtype, long long ldo, float* s, long long lds, int T, int H, cudaStream_t stream) {
+// x [T,H] in place; d [T,H] or null; gate: g [T,H] or gc float [H] or neither; w1 or null; out [T,H] of out_kind (0 float, 1 bfloat16,
+// 2 e4m3 with scales s [T][groups of H], 3 none); every matrix's rows dense at a stride of its own.  (One record, field for field as
+// kernels/ops.py packs it.)
+struct GatedNormsArgs {
+    const void *x, *d, *g, *gc, *w1, *w2, *out, *s, *stream;
+    long long ldx, ldd, ldg, ldo, lds;
+    int x_dtype, d_dtype, g_dtype, out_kind, T, H;
+    float c, e1, e2;
+};
+ACV_API int acv_add_gated_norms(const GatedNormsArgs* a) {
+    const int T = a->T, H = a->H;
     if (T <= 0 || H <= 0) return 0;
-    if ((x_dtype | d_dtype | g_dtype) & ~1) return ACV_ERR_DTYPE;
-    if (out && ((unsigned)out_dtype > 2u || !w2 || (out_dtype == 2 && !s))) return ACV_ERR_DTYPE;
+    if ((a->x_dtype | a->d_dtype | a->g_dtype) & ~1) return ACV_ERR_DTYPE;
+    if ((unsigned)a->out_kind > 3u || (a->out_kind < 3 && (!a->out || !a->w2)) || (a->out_kind == 2 && !a->s)) return ACV_ERR_DTYPE;
     GnParams p = {};
-    p.x = x; p.d = d; p.g = g; p.gc = g ? nullptr : gc; p.w1 = d ? w1 : nullptr; p.w2 = out ? w2 : nullptr; p.out = out; p.s = s;
-    p.ldx = ldx; p.ldd = ldd; p.ldg = ldg; p.ldo = ldo; p.lds = lds; p.H = H;
-    p.x_f32 = x_dtype == ACV_F32; p.d_f32 = d_dtype == ACV_F32; p.g_f32 = g_dtype == ACV_F32; p.out_kind = out ? out_dtype : 3;
-    p.c = c; p.e1 = e1; p.e2 = e2;
+    p.x = const_cast<void*>(a->x); p.d = a->d; p.g = a->g; p.gc = a->g ? nullptr : (const float*)a->gc;
+    p.w1 = a->d ? (const float*)a->w1 : nullptr; p.w2 = a->out_kind < 3 ? (const float*)a->w2 : nullptr;
+    p.out = const_cast<void*>(a->out); p.s = (float*)const_cast<void*>(a->s);
+    p.ldx = a->ldx; p.ldd = a->ldd; p.ldg = a->ldg; p.ldo = a->ldo; p.lds = a->lds; p.H = H;
+    p.x_f32 = a->x_dtype == ACV_F32; p.d_f32 = a->d_dtype == ACV_F32; p.g_f32 = a->g_dtype == ACV_F32; p.out_kind = a->out_kind;
+    p.c = a->c; p.e1 = a->e1; p.e2 = a->e2;
     const int ob = p.out_kind == 0 ? 4 : p.out_kind == 1 ? 2 : 1;
-    const bool vec = H % 8 == 0 && fp8_rows_aligned(x, ldx, p.x_f32 ? 4 : 2, 16) && (!d || fp8_rows_aligned(d, ldd, p.d_f32 ? 4 : 2, 16)) &&
-                     (!g || fp8_rows_aligned(g, ldg, p.g_f32 ? 4 : 2, 16)) && (!out || fp8_rows_aligned(out, ldo, ob, p.out_kind == 2 ? 8 : 16)) &&
+    const bool vec = H % 8 == 0 && fp8_rows_aligned(p.x, p.ldx, p.x_f32 ? 4 : 2, 16) && (!p.d || fp8_rows_aligned(p.d, p.ldd, p.d_f32 ? 4 : 2, 16)) &&
+                     (!p.g || fp8_rows_aligned(p.g, p.ldg, p.g_f32 ? 4 : 2, 16)) &&
+                     (p.out_kind == 3 || fp8_rows_aligned(p.out, p.ldo, ob, p.out_kind == 2 ? 8 : 16)) &&
                      !(((uintptr_t)p.gc | (uintptr_t)p.w1 | (uintptr_t)p.w2) & 15);
+    const cudaStream_t stream = (cudaStream_t)const_cast<void*>(a->stream);
     return vec ? gn_launch<true>(p, T, stream) : gn_launch<false>(p, T, stream);
 }

@@ -3,17 +3,21 @@
 //   y[t][n] = sum over groups g of 128 k of  sx[t][g] sw[n / 128][g] P_g[t][n],   P_g[t][n] = sum over k in g of qx[t][k] qw[n][k]
 //
 // P_g is what tcgen05.mma (kind::f8f6f4, operands staged by TMA, 128-byte swizzle: a k-block of 128 is one swizzle row) leaves in
-// tensor memory for one k-block.  It cannot stay there: its scales differ from k-block to k-block.  Tensor memory holds two such
-// partial tiles; while the tensor core fills one, eight epilogue warps fetch the other and add it, times its scales, to the float
+// tensor memory for one k-block.  It cannot stay there: its scales differ from k-block to k-block.  Tensor memory holds several such
+// partial tiles; while the tensor core fills one, the epilogue warps fetch another and add it, times its scales, to the float
 // sums that they hold in registers (a fused multiply-add for each output and k-block, two at a time as fma.rn.f32x2).  Tokens are
-// the rows (a lane holds one, so sx is a number of the thread's), features the columns (128 of them, one block row of sw, to a
-// thread or two).
+// the rows (a lane holds one, so sx is a number of the thread's), features the columns, 64 or 128 of them to a thread.
 //
 // Two forms.  Pairs of CTAs on tiles of 256 x 256 (cta_group::2), persistent, for many tokens: a CTA loads 128 rows of each operand
 // for a k-block, 32 KB for 512 cycles of tensor core.  And single CTAs on tiles of 128 x BN, one each, for fewer: K may be split over
 // the CTAs of a cluster, whose sums meet through its shared memory, in rank order, so the result does not depend on timing.
 //
-// Warps: 0 loads, 1 issues the products, 2..9 are the epilogue, two to each quarter of the lanes.  Every wait on an mbarrier is
+// What bounds the many-token form beside the tensor core is that hand-over, once for each k-block: from the products' end until the
+// epilogue warps of both CTAs have fetched the partial tile and the issuing thread knows it.  With two partial tiles of 256 columns
+// the tensor core waited for it (4096 x 4096 x 12288 in 211 us, and in as many without any fetch or sum; 155 us with nobody to wait
+// for); with four of 128 columns three others are under way meanwhile.
+//
+// Warps: 0 loads, 1 issues the products, from 2 on they are the epilogue, each a quarter of the lanes.  Every wait on an mbarrier is
 // bounded; when one runs out the kernel records where in `status`, all roles leave their loops, the loads in flight are waited for
 // (with a limit), tensor memory is freed and the kernel returns.
 #include "fp8.cuh"
@@ -21,7 +25,6 @@
 #include "tensor_map.h"
 #include "gemm_fp8.h"
 
-#define FT_THREADS 320
 #define FT_ROWS 128                         // rows of an operand tile = bytes of a k-block's row
 #define FT_TILE (FT_ROWS * FT_ROWS)         // bytes of an operand tile of 128 rows
 
@@ -31,7 +34,7 @@ struct Fp8TcParams {
     long long ldsx, ldsw, ldsw2, ldo, ldso;
     void* out;
     float* so;
-    int out_f32, out_vec;                   // out_vec: rows of out take 16-byte stores
+    int out_f32, out_vec, sx_vec;           // _vec: rows of out take 16-byte stores, those of sx 16-byte loads
     int tiles_m, tiles_n, group, stages, splits, kb_per_split, early_w;
     int* status;
     unsigned int wait_limit;                // of polls; less and a k-block whose loads are left out (skip_kb >= 0) in the test of the waits only
@@ -41,20 +44,23 @@ struct Fp8TcParams {
 __device__ __forceinline__ uint32_t ft_idesc(int n, int m) {        // float accumulator, e4m3 operands (type 0), both K-major
     return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// One lane of a converged warp.  The issuing warp runs its loop as a whole and lets this lane issue: what the products need is then
+// known to be the warp's and is kept in uniform registers.  (A loop run by one lane alone moved every descriptor there first: 600
+// cycles a k-block, where the tensor core needs 512 for the largest.)
+__device__ __forceinline__ bool ft_elect() {
+    uint32_t yes;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
+    return yes != 0;
+}
+__device__ __forceinline__ int ft_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
 template <bool PAIR>
-__device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
     if (PAIR)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
-            ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
     else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t}"
-            ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                     ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
 }
 // the registers of a load are what its wait hands over: nothing that reads them moves in front of it
 __device__ __forceinline__ void ft_wait_ld(uint32_t (&r)[16]) {
@@ -70,16 +76,21 @@ __device__ __forceinline__ uint64_t ft_both(float v) {
     asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(v)));
     return r;
 }
+__device__ __forceinline__ uint64_t ft_pair(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(lo)), "r"(__float_as_uint(hi)));
+    return r;
+}
 __device__ __forceinline__ float2 ft_floats(uint64_t v) {
     uint32_t lo, hi;
     asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
     return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
 
-// sums[0 .. 8 PIECES) += scale * the tile's 16 PIECES columns, a piece from `first` + 16 i (from `second` + 16 (i - PIECES / 2) in the
-// second half); the next piece is on its way while one is added
+// sums[0 .. 8 PIECES) += scales * 16 PIECES columns of this lane's row, the first half of them from `first`, the others from `second`;
+// a piece of sixteen is on its way while the one before is added
 template <int PIECES>
-__device__ __forceinline__ void ft_add_tile(uint64_t (&sums)[8 * PIECES], uint32_t first, uint32_t second, float scale1, float scale2) {
+__device__ __forceinline__ void ft_add_tile(uint64_t* sums, uint32_t first, uint32_t second, float scale1, float scale2) {
     const uint64_t s1 = ft_both(scale1), s2 = ft_both(scale2);
     uint32_t r[2][16];
     tc_ld16_nowait(first, r[0]);
@@ -92,6 +103,46 @@ __device__ __forceinline__ void ft_add_tile(uint64_t (&sums)[8 * PIECES], uint32
         if (i + 1 < PIECES) ft_wait_ld(r[(i + 1) & 1]);
     }
 }
+
+// A row's scales, four k-blocks at a time and four ahead of their use: lanes hold rows, so a load touches 32 lines whatever its width
+// (one number at a time, those lookups took 1000 cycles a k-block, twice what the tensor core needs).
+struct FtRowScales {
+    const float* at;
+    int left, vec;
+    float now[4], next[4];
+    __device__ __forceinline__ void fetch(float (&v)[4]) {
+        if (vec && left >= 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(at));
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = i < left ? __ldg(at + i) : 0.f;
+        }
+        at += 4;
+        left -= 4;
+    }
+    __device__ __forceinline__ void begin(const float* row, int count, int aligned) {
+        at = row;
+        left = count;
+        vec = aligned;
+        fetch(now);
+        fetch(next);
+    }
+    // the scale of the i-th k-block, i = 0, 1, 2, ...
+    __device__ __forceinline__ float take(int i) {
+        const float v = now[0];
+        if ((i & 3) == 3) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) now[j] = next[j];
+            fetch(next);
+        } else {
+            now[0] = now[1];
+            now[1] = now[2];
+            now[2] = now[3];
+        }
+        return v;
+    }
+};
 
 // sixteen neighbouring outputs of a row
 __device__ __forceinline__ void ft_store16(const Fp8TcParams& p, int row, int n, const uint64_t* v) {
@@ -144,12 +195,12 @@ __device__ __forceinline__ void ft_drain(uint32_t full0, int stages, int asked, 
     }
 }
 
-// the epilogue's wait, by a whole warp: true for all of its lanes where it ran out for one
-__device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Fp8TcParams& p) {
+// a wait by a whole warp: true for all of its lanes where it ran out for one
+__device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Fp8TcParams& p, int code = 4) {
     const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit));
     if (!ok && (threadIdx.x & 31) == 0) {
         *abort_flag = 1;
-        atomicExch(p.status, 4);
+        atomicExch(p.status, code);
     }
     return !ok;
 }
@@ -157,29 +208,32 @@ __device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, vo
 // ----------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256
 #define FP_STAGE (2 * FT_TILE)              // a CTA's share of a k-block: 128 rows of tokens, 128 of weights
 #define FP_MAX_STAGES 6
+#define FP_THREADS 320
+#define FP_SLOTS 2                          // partial tiles in tensor memory
 
 // GATED: the tile's columns are 128 units' gate rows (the leader's half of the weight tile) and the same units' up rows (the other's).
 template <bool GATED>
-__global__ void __launch_bounds__(FT_THREADS, 1)
+__global__ void __launch_bounds__(FP_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_w2, const Fp8TcParams p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = smem_raw + ((1024u - (gt_smem(smem_raw) & 1023u)) & 1023u);
     const int STAGES = p.stages;
     const uint32_t tiles_addr = gt_smem(tiles);
-    // barriers: full[STAGES] (the leader's count both CTAs' bytes), empty[STAGES], tmem_full[2], tmem_empty[2] (the leader's)
-    const uint32_t full0 = tiles_addr + STAGES * FP_STAGE, empty0 = full0 + 8 * STAGES, tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16;
+    // barriers: full[STAGES] (the leader's count both CTAs' bytes), empty[STAGES], tmem_full[SLOTS], tmem_empty[SLOTS] (the leader's)
+    const uint32_t full0 = tiles_addr + STAGES * FP_STAGE, empty0 = full0 + 8 * STAGES, tfull0 = empty0 + 8 * STAGES;
+    const uint32_t tempty0 = tfull0 + 8 * FP_SLOTS;
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_s;
     __shared__ uint32_t most[GATED ? 2 : 1][2][FT_ROWS];
     __shared__ __align__(8) uint64_t met[4];            // the two warps of a quarter of the lanes tell each other their maxima
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = ft_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, n_items = p.tiles_m * p.tiles_n;
     if (threadIdx.x == 0) {
         abort_s = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 16); }
+        for (int b = 0; b < FP_SLOTS; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 16); }
         for (int q = 0; q < 4; ++q) mbar_init(gt_smem(&met[q]), 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -198,7 +252,9 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         if (lane == 0) {
             const uint32_t lead_full0 = cluster_map(full0, 0);
             const CUtensorMap* weights = GATED && rank == 1 ? &map_w2 : &map_w;
-            auto weight_row = [&](int tb) { return GATED ? tb * FT_ROWS : tb * 2 * FT_ROWS + (int)rank * FT_ROWS; };
+            auto load_w = [&](uint32_t dst, uint32_t bar, int kb, int tb) {
+                tma_load_2d_pair(dst, weights, bar, kb * FT_ROWS, GATED ? tb * FT_ROWS : tb * 2 * FT_ROWS + (int)rank * FT_ROWS);
+            };
             int early = 0, asked = 0;
             if (p.early_w && pair < n_items) {
                 int ta, tb;
@@ -206,7 +262,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 early = min(STAGES, p.n_kb);
                 for (int i = 0; i < early; ++i) {
                     if (rank == 0) mbar_expect_tx(full0 + 8 * i, 2 * FP_STAGE);
-                    tma_load_2d_pair(tiles_addr + i * FP_STAGE + FT_TILE, weights, lead_full0 + 8 * i, i * FT_ROWS, weight_row(tb));
+                    load_w(tiles_addr + i * FP_STAGE + FT_TILE, lead_full0 + 8 * i, i, tb);
                 }
             }
             pdl_wait();
@@ -227,40 +283,43 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                     ++asked;
                     if (kb == p.skip_kb) continue;
                     tma_load_2d_pair(dst, &map_x, lead_full0 + 8 * s, kb * FT_ROWS, ta * 2 * FT_ROWS + (int)rank * FT_ROWS);
-                    if (!half_done) tma_load_2d_pair(dst + FT_TILE, weights, lead_full0 + 8 * s, kb * FT_ROWS, weight_row(tb));
+                    if (!half_done) load_w(dst + FT_TILE, lead_full0 + 8 * s, kb, tb);
                 }
             }
             if (abort_s && rank == 0) ft_drain(full0, STAGES, asked, p.wait_limit);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             pdl_wait();         // (the first tokens come after it: the wait for them starts there)
             const uint32_t idesc = ft_idesc(2 * FT_ROWS, 2 * FT_ROWS);
-            const uint32_t a_lo0 = umma_desc_lo(tiles_addr), b_lo0 = umma_desc_lo(tiles_addr + FT_TILE);
-            uint32_t turn = 0, ph = 0, s_lo = 0;
+            const uint64_t a0 = umma_desc(tiles_addr), b0 = umma_desc(tiles_addr + FT_TILE);
+            uint32_t turn = 0, ph = 0;
             int s = 0;
             bool failed = false;
-            for (int item = pair; item < n_items && !abort_s && !failed; item += n_pairs) {
+            for (int item = pair; item < n_items && !failed; item += n_pairs) {
                 for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
-                    const uint32_t buf = turn & 1, use = turn >> 1;
-                    if (!mbar_wait(full0 + 8 * s, ph, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 3); failed = true; break; }
-                    if (!mbar_wait(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 2); failed = true; break; }
+                    const uint32_t slot = turn % FP_SLOTS, use = turn / FP_SLOTS;
+                    failed = ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3) || ft_warp_failed(tempty0 + 8 * slot, (use & 1) ^ 1, &abort_s, p, 2);
+                    if (failed) break;
                     tc_fence_after();
-                    const uint32_t d = tmem_base + buf * 2 * FT_ROWS, a_lo = a_lo0 + s_lo, b_lo = b_lo0 + s_lo;
+                    if (ft_elect()) {
+                        const uint64_t a = a0 + (uint64_t)(s * (FP_STAGE >> 4)), b = b0 + (uint64_t)(s * (FP_STAGE >> 4));
+                        const uint32_t d = tmem_base + slot * 2 * FT_ROWS;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) ft_mma<true>(d, a_lo + 2 * k, b_lo + 2 * k, idesc, k > 0);
-                    tc_commit_pair(empty0 + 8 * s, 3);
-                    tc_commit_pair(tfull0 + 8 * buf, 3);
-                    ++s; s_lo += FP_STAGE >> 4;
-                    if (s == STAGES) { s = 0; s_lo = 0; ph ^= 1; }
+                        for (int k = 0; k < 4; ++k) ft_mma<true>(d, a + 2 * k, b + 2 * k, idesc, k > 0);
+                        tc_commit_pair(tfull0 + 8 * slot, 3);
+                        tc_commit_pair(empty0 + 8 * s, 3);
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) { s = 0; ph ^= 1; }
                 }
             }
         }
     } else {
-        const int wq = warp & 3, half = (warp - 2) >> 2;
+        const int wq = warp & 3, part = (warp - 2) >> 2;
         pdl_wait();
         const uint32_t lead_tempty0 = cluster_map(tempty0, 0);
-        const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16);
+        const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16) + part * (GATED ? 64 : FT_ROWS);
         uint32_t turn = 0, parity = 0;
         // (a warp gives up as a whole: its loads from tensor memory and its exchanges are the whole warp's)
         bool failed = false;
@@ -270,70 +329,74 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             const int row = ta * 2 * FT_ROWS + (int)rank * FT_ROWS + wq * 32 + lane;
             // (rows and blocks that do not exist have products of zeros: any scale that does exist will do)
             const float* sx = p.sx + (size_t)min(row, p.M - 1) * p.ldsx;
-            const int block = GATED ? tb : min(tb * 2 + half, (p.N - 1) / FT_ROWS);
+            const int block = GATED ? tb : min(tb * 2 + part, (p.N - 1) / FT_ROWS);
             const float *sw = p.sw + (size_t)block * p.ldsw, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : nullptr;
             uint64_t sums[64];
 #pragma unroll
             for (int i = 0; i < 64; ++i) sums[i] = 0;
-            float next_x = __ldg(sx), next_w = __ldg(sw), next_w2 = GATED ? __ldg(sw2) : 0.f;
+            FtRowScales xs;
+            xs.begin(sx, p.n_kb, p.sx_vec);
+            float next_w = __ldg(sw), next_w2 = GATED ? __ldg(sw2) : 0.f;
             for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
-                const float a = next_x, b = next_w, b2 = next_w2;
+                const float x = xs.take(kb), s1 = x * next_w, s2 = GATED ? x * next_w2 : s1;
                 if (kb + 1 < p.n_kb) {
-                    next_x = __ldg(sx + kb + 1);
                     next_w = __ldg(sw + kb + 1);
                     if (GATED) next_w2 = __ldg(sw2 + kb + 1);
                 }
-                const uint32_t buf = turn & 1, use = turn >> 1;
-                failed = ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p);
+                const uint32_t slot = turn % FP_SLOTS, use = turn / FP_SLOTS;
+                failed = ft_warp_failed(tfull0 + 8 * slot, use & 1, &abort_s, p);
                 if (failed) break;
                 tc_fence_after();
-                const uint32_t t = taddr + buf * 2 * FT_ROWS;
-                if (GATED) ft_add_tile<8>(sums, t + half * 64, t + FT_ROWS + half * 64, a * b, a * b2);
-                else ft_add_tile<8>(sums, t + half * FT_ROWS, t + half * FT_ROWS + 64, a * b, a * b);
+                const uint32_t t = taddr + slot * 2 * FT_ROWS;
+                ft_add_tile<8>(sums, t, t + (GATED ? FT_ROWS : 64), s1, s2);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    if (rank == 0) mbar_arrive(tempty0 + 8 * buf);
-                    else mbar_arrive_remote(lead_tempty0 + 8 * buf);
+                    if (rank == 0) mbar_arrive(tempty0 + 8 * slot);
+                    else mbar_arrive_remote(lead_tempty0 + 8 * slot);
                 }
             }
             if (failed) break;
             if (!GATED) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ft_store16(p, row, tb * 2 * FT_ROWS + half * FT_ROWS + 16 * i, sums + 8 * i);
+                for (int i = 0; i < 8; ++i)
+                    ft_store16(p, row, tb * 2 * FT_ROWS + part * FT_ROWS + 16 * i, sums + 8 * i);
             } else {
-                // silu(gate) * up of 64 units; the other 64 of the group are the partner warp's
+                // silu(gate) * up of 64 units, in the place of the gates' sums; the other 64 of the group are the partner warp's
                 uint32_t m = 0;
-                float act[64];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     const float2 g = ft_floats(sums[i]), u = ft_floats(sums[32 + i]);
-                    act[2 * i] = silu_f32<float>(g.x) * u.x;
-                    act[2 * i + 1] = silu_f32<float>(g.y) * u.y;
-                    m = max(m, max(fp8_magnitude(act[2 * i]), fp8_magnitude(act[2 * i + 1])));
+                    const float a = silu_f32<float>(g.x) * u.x, b = silu_f32<float>(g.y) * u.y;
+                    m = max(m, max(fp8_magnitude(a), fp8_magnitude(b)));
+                    sums[i] = ft_pair(a, b);
                 }
-                most[parity][half][wq * 32 + lane] = m;
+                most[parity][part][wq * 32 + lane] = m;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(gt_smem(&met[wq]));
                 failed = ft_warp_failed(gt_smem(&met[wq]), parity, &abort_s, p);
                 if (failed) break;
-                const Fp8Scale k = fp8_scale(max(m, most[parity][half ^ 1][wq * 32 + lane]));
+                const Fp8Scale k = fp8_scale(max(m, most[parity][part ^ 1][wq * 32 + lane]));
                 parity ^= 1;
-                const int u0 = tb * FT_ROWS + half * 64;
                 if (row < p.M) {
-                    if (half == 0) p.so[(size_t)row * p.ldso + tb] = k.s;
-                    uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + (size_t)row * p.ldo + u0;
+                    if (part == 0) p.so[(size_t)row * p.ldso + tb] = k.s;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
+                        const int u = tb * FT_ROWS + part * 64 + i * 16;
+                        const uint64_t* v = sums + 8 * i;
+                        uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + (size_t)row * p.ldo + u;
                         uint32_t w[4];
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) w[c] = fp8_pack4(act[16 * i + 4 * c], act[16 * i + 4 * c + 1], act[16 * i + 4 * c + 2], act[16 * i + 4 * c + 3], k.r);
-                        if (p.out_vec && u0 + 16 * i + 16 <= p.N) {
-                            *reinterpret_cast<uint4*>(o + 16 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        for (int c = 0; c < 4; ++c) {
+                            const float2 x = ft_floats(v[2 * c]), y = ft_floats(v[2 * c + 1]);
+                            w[c] = fp8_pack4(x.x, x.y, y.x, y.y, k.r);
+                        }
+                        if (p.out_vec && u + 16 <= p.N) {
+                            *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2], w[3]);
                         } else {
 #pragma unroll
                             for (int c = 0; c < 16; ++c)
-                                if (u0 + 16 * i + c < p.N) o[16 * i + c] = (uint8_t)(w[c >> 2] >> (8 * (c & 3)));
+                                if (u + c < p.N) o[c] = (uint8_t)(w[c >> 2] >> (8 * (c & 3)));
                         }
                     }
                 }
@@ -354,9 +417,13 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 template <int BN>
 struct Fp8TileShape {
     static constexpr int STAGE = FT_TILE + BN * FT_ROWS;
-    static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
+    static constexpr int SLOTS = BN <= 128 ? 4 : 2;                 // partial tiles in tensor memory
+    static constexpr int TMEM = SLOTS * BN;
     static constexpr int LD = BN + 4;                               // floats of a row of the summed tile: sixteen-byte stores of eight rows meet no bank twice
     static constexpr int SUMS = FT_ROWS * LD * 4;
+    static constexpr int COLS = BN == 256 ? 128 : 64;               // of an epilogue thread
+    static constexpr int WARPS = 4 * BN / COLS;                     // of the epilogue
+    static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int smem(int stages) { return 1024 + (stages * STAGE > SUMS ? stages * STAGE : SUMS) + 256; }
 };
 
@@ -368,7 +435,7 @@ __device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
 
 // GATED: BN is 256, the columns are 128 units' gate rows and their up rows, and a row of the result is a whole group.
 template <int BN, bool GATED>
-__global__ void __launch_bounds__(FT_THREADS, 1)
+__global__ void __launch_bounds__(Fp8TileShape<BN>::THREADS, 1)
 gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_w2, const Fp8TcParams p) {
     using S = Fp8TileShape<BN>;
@@ -377,16 +444,16 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const int STAGES = p.stages;
     const uint32_t tiles_addr = gt_smem(tiles);
     const uint32_t full0 = tiles_addr + (STAGES * S::STAGE > S::SUMS ? STAGES * S::STAGE : S::SUMS), empty0 = full0 + 8 * STAGES;
-    const uint32_t tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 16;
+    const uint32_t tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 8 * S::SLOTS;
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_s;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = ft_warp(), lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, ta = tile % p.tiles_m, tb = tile / p.tiles_m;
     const int kb0 = split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.n_kb);
     if (threadIdx.x == 0) {
         abort_s = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
-        for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 8); }
+        for (int b = 0; b < S::SLOTS; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, S::WARPS); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -433,53 +500,53 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             if (abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            pdl_wait();
-            const uint32_t idesc = ft_idesc(BN, FT_ROWS);
-            const uint32_t a_lo0 = umma_desc_lo(tiles_addr), b_lo0 = umma_desc_lo(tiles_addr + FT_TILE);
-            uint32_t turn = 0, ph = 0, s_lo = 0;
-            int s = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++turn) {
-                const uint32_t buf = turn & 1, use = turn >> 1;
-                if (!mbar_wait(full0 + 8 * s, ph, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 3); break; }
-                if (!mbar_wait(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 2); break; }
-                tc_fence_after();
-                const uint32_t d = tmem_base + buf * BN, a_lo = a_lo0 + s_lo, b_lo = b_lo0 + s_lo;
+        pdl_wait();
+        const uint32_t idesc = ft_idesc(BN, FT_ROWS);
+        const uint64_t a0 = umma_desc(tiles_addr), b0 = umma_desc(tiles_addr + FT_TILE);
+        uint32_t turn = 0, ph = 0;
+        int s = 0;
+        for (int kb = kb0; kb < kb1; ++kb, ++turn) {
+            const uint32_t buf = turn % S::SLOTS, use = turn / S::SLOTS;
+            if (ft_warp_failed(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p, 2) || ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) break;
+            tc_fence_after();
+            if (ft_elect()) {
+                const uint64_t a = a0 + (uint64_t)(s * (S::STAGE >> 4)), b = b0 + (uint64_t)(s * (S::STAGE >> 4));
+                const uint32_t d = tmem_base + buf * BN;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) ft_mma<false>(d, a_lo + 2 * k, b_lo + 2 * k, idesc, k > 0);
-                tc_commit(empty0 + 8 * s);
+                for (int k = 0; k < 4; ++k) ft_mma<false>(d, a + 2 * k, b + 2 * k, idesc, k > 0);
                 tc_commit(tfull0 + 8 * buf);
-                ++s; s_lo += S::STAGE >> 4;
-                if (s == STAGES) { s = 0; s_lo = 0; ph ^= 1; }
+                tc_commit(empty0 + 8 * s);
             }
+            __syncwarp();
+            if (++s == STAGES) { s = 0; ph ^= 1; }
         }
     } else {
-        constexpr int PIECES = BN / 32;             // of sixteen columns: a thread's half of the tile
-        const int wq = warp & 3, half = (warp - 2) >> 2;
+        const int wq = warp & 3, part = (warp - 2) >> 2;
         pdl_wait();
         const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16);
         const int r = wq * 32 + lane;
         const float* sx = p.sx + (size_t)min(row_here + r, p.M - 1) * p.ldsx;
-        const int block = GATED ? tb : min((tb * BN + (BN > FT_ROWS ? half * FT_ROWS : 0)) / FT_ROWS, (p.N - 1) / FT_ROWS);
+        const int block = GATED ? tb : min(tb * BN / FT_ROWS, (p.N - 1) / FT_ROWS);
         const float *sw = p.sw + (size_t)block * p.ldsw, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : nullptr;
-        uint64_t sums[8 * PIECES];
+        uint64_t sums[S::COLS / 2];
 #pragma unroll
-        for (int i = 0; i < 8 * PIECES; ++i) sums[i] = 0;
-        float next_x = __ldg(sx + kb0), next_w = __ldg(sw + kb0), next_w2 = GATED ? __ldg(sw2 + kb0) : 0.f;
+        for (int i = 0; i < S::COLS / 2; ++i) sums[i] = 0;
+        FtRowScales xs;
+        xs.begin(sx + kb0, kb1 - kb0, p.sx_vec && !(kb0 & 3));
+        float next_w = __ldg(sw + kb0), next_w2 = GATED ? __ldg(sw2 + kb0) : 0.f;
         uint32_t turn = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++turn) {
-            const float a = next_x, b = next_w, b2 = next_w2;
+            const float a = xs.take((int)turn), b = next_w, b2 = next_w2;
             if (kb + 1 < kb1) {
-                next_x = __ldg(sx + kb + 1);
                 next_w = __ldg(sw + kb + 1);
                 if (GATED) next_w2 = __ldg(sw2 + kb + 1);
             }
-            const uint32_t buf = turn & 1, use = turn >> 1;
+            const uint32_t buf = turn % S::SLOTS, use = turn / S::SLOTS;
             if (ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p)) break;
             tc_fence_after();
             const uint32_t t = taddr + buf * BN;
-            if (GATED) ft_add_tile<PIECES>(sums, t + half * 64, t + FT_ROWS + half * 64, a * b, a * b2);
-            else ft_add_tile<PIECES>(sums, t + half * (BN / 2), t + half * (BN / 2) + BN / 4, a * b, a * b);
+            if (GATED) ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + FT_ROWS + part * 64, a * b, a * b2);
+            else ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + part * 64 + 32, a * b, a * b);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(tempty0 + 8 * buf);
@@ -489,9 +556,9 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         if (!abort_s && row_here + r < p.M) {
             float* to = reinterpret_cast<float*>(tiles) + r * S::LD;
 #pragma unroll
-            for (int i = 0; i < 4 * PIECES; ++i) {
+            for (int i = 0; i < S::COLS / 4; ++i) {
                 const float2 lo = ft_floats(sums[2 * i]), hi = ft_floats(sums[2 * i + 1]);
-                const int c = GATED ? (i < 2 * PIECES ? half * 64 + 4 * i : FT_ROWS + half * 64 + 4 * (i - 2 * PIECES)) : half * (BN / 2) + 4 * i;
+                const int c = i < 16 ? part * 64 + 4 * i : FT_ROWS + part * 64 + 4 * (i - 16);      // (the second 64: the up rows')
                 *reinterpret_cast<float4*>(to + c) = make_float4(lo.x, lo.y, hi.x, hi.y);
             }
         }
@@ -504,7 +571,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const uint32_t own = tiles_addr;
     if (!abort_s) {
 #pragma unroll 1
-        for (int r = split + p.splits * warp; r < rows; r += p.splits * (FT_THREADS / 32)) {
+        for (int r = split + p.splits * warp; r < rows; r += p.splits * (S::THREADS / 32)) {
             auto sum4 = [&](int c) {
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 const uint32_t at = own + (uint32_t)(r * S::LD + c) * 4;
@@ -614,7 +681,7 @@ static int ft_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CU
         if (resident <= 0) {
             cudaLaunchConfig_t lc = {};
             lc.gridDim = dim3(2 * (sms / 2));
-            lc.blockDim = dim3(FT_THREADS);
+            lc.blockDim = dim3(FP_THREADS);
             lc.dynamicSmemBytes = smem;
             cudaLaunchAttribute attr[1];
             attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -634,7 +701,7 @@ static int ft_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CU
     const long long items = (long long)p.tiles_m * p.tiles_n;
     if (items > 0x7fffffff) return ACV_ERR_SIZE;
     const int pairs = (int)(items < resident ? items : resident);
-    acv_launch_cluster(PDL_GEMM, dim3(2, 1, 1), kernel, dim3(2 * pairs), dim3(FT_THREADS), smem, stream, mx, mw, mw2, p);
+    acv_launch_cluster(PDL_GEMM, dim3(2, 1, 1), kernel, dim3(2 * pairs), dim3(FP_THREADS), smem, stream, mx, mw, mw2, p);
     return acv_launch_status();
 }
 
@@ -655,7 +722,7 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
     if (const int rc = acv_ensure_smem(cfg, kernel, smem)) return rc;
     const long long ctas = (long long)p.tiles_m * p.tiles_n * p.splits;
     if (ctas > 0x7fffffff) return ACV_ERR_SIZE;
-    acv_launch_cluster(PDL_GEMM, dim3(p.splits, 1, 1), kernel, dim3((unsigned)ctas), dim3(FT_THREADS), smem, stream, mx, mw, mw2, p);
+    acv_launch_cluster(PDL_GEMM, dim3(p.splits, 1, 1), kernel, dim3((unsigned)ctas), dim3(S::THREADS), smem, stream, mx, mw, mw2, p);
     return acv_launch_status();
 }
 
@@ -684,6 +751,7 @@ static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cud
     p.sx = o.sx; p.sw = o.sw; p.sw2 = o.sw2; p.ldsx = o.ldsx; p.ldsw = o.ldsw; p.ldsw2 = o.ldsw2; p.ldo = o.ldo; p.ldso = o.ldso;
     p.out = o.out; p.so = o.so; p.out_f32 = o.out_f32; p.early_w = flags & 1; p.status = status;
     p.out_vec = fp8_rows_aligned(o.out, o.ldo, gated ? 1 : o.out_f32 ? 4 : 2, 16);
+    p.sx_vec = fp8_rows_aligned(o.sx, o.ldsx, 4, 16);
     p.wait_limit = g_test_wait_limit ? g_test_wait_limit : GT_WAIT_LIMIT;
     p.skip_kb = g_test_skip_kb;
     g_test_wait_limit = 0; g_test_skip_kb = -1;
@@ -703,27 +771,24 @@ static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cud
     }
 }
 
-// x [M,K] bytes, sx [M][groups of K]; w [N,K] bytes, sw [blocks of N][groups of K]; out [M,N] float or bfloat16; every matrix's rows at a
-// stride of its own, those of x and w on 16 bytes.  flags: 1 the weights were written long before, they may be read while the kernel
-// in front still runs.  plan: 0, or kind | bn << 4 | splits << 16.  status: one int, 0 unless a bounded wait ran out.
-ACV_API int acv_linear_fp8(const void* x, long long ldx, const float* sx, long long ldsx, const void* w, long long ldw, const float* sw,
-                           long long ldsw, void* out, long long ldo, int out_f32, int M, int N, int K, int flags, int plan, int* status,
-                           int sms, cudaStream_t stream) {
+// A call's arguments as one record (a caller through a foreign-function interface pays for each argument by itself), field for field as
+// kernels/ops.py packs them.  x [M,K] bytes, sx [M][groups of K]; w [N,K] bytes, sw [blocks of N][groups of K]; out [M,N] float or
+// bfloat16; every matrix's rows at a stride of its own, those of x and w on 16 bytes.  With w2, sw2 and so, the gated form: w and w2 are
+// gate and up rows, out [M,N] bytes = silu(gate) * up by its own scales so [M][groups of N].  flags: 1 the weights were written
+// long before, they may be read while the kernel in front still runs.  plan: 0, or kind | bn << 4 | splits << 16.  status: one int,
+// 0 unless a bounded wait ran out.
+struct Fp8LinearArgs {
+    const void *x, *sx, *w, *sw, *out, *w2, *sw2, *so, *status, *stream;
+    long long ldx, ldsx, ldw, ldsw, ldo, ldw2, ldsw2, ldso;
+    int M, N, K, out_f32, flags, plan, sms;
+};
+ACV_API int acv_linear_fp8(const Fp8LinearArgs* a) {
     Fp8Operands o = {};
-    o.x = (const uint8_t*)x; o.w = (const uint8_t*)w; o.sx = sx; o.sw = sw; o.out = out;
-    o.ldx = ldx; o.ldw = ldw; o.ldo = ldo; o.ldsx = ldsx; o.ldsw = ldsw; o.M = M; o.N = N; o.K = K; o.out_f32 = out_f32;
-    return ft_run(o, flags, plan, status, sms, stream);
-}
-
-// The same for gate rows w and up rows w2 [N,K] each: out [M,N] bytes = silu(gate) * up by its own scales so [M][groups of N].
-ACV_API int acv_linear_fp8_swiglu(const void* x, long long ldx, const float* sx, long long ldsx, const void* w, long long ldw, const float* sw,
-                                  long long ldsw, const void* w2, long long ldw2, const float* sw2, long long ldsw2, void* out,
-                                  long long ldo, float* so, long long ldso, int M, int N, int K, int flags, int plan, int* status, int sms,
-                                  cudaStream_t stream) {
-    if (!w2) return ACV_ERR_SIZE;
-    Fp8Operands o = {};
-    o.x = (const uint8_t*)x; o.w = (const uint8_t*)w; o.w2 = (const uint8_t*)w2; o.sx = sx; o.sw = sw; o.sw2 = sw2; o.out = out; o.so = so;
-    o.ldx = ldx; o.ldw = ldw; o.ldw2 = ldw2; o.ldo = ldo; o.ldsx = ldsx; o.ldsw = ldsw; o.ldsw2 = ldsw2; o.ldso = ldso;
-    o.M = M; o.N = N; o.K = K;
-    return ft_run(o, flags, plan, status, sms, stream);
+    o.x = (const uint8_t*)a->x; o.w = (const uint8_t*)a->w; o.w2 = (const uint8_t*)a->w2;
+    o.sx = (const float*)a->sx; o.sw = (const float*)a->sw; o.sw2 = (const float*)a->sw2;
+    o.out = const_cast<void*>(a->out); o.so = (float*)const_cast<void*>(a->so);
+    o.ldx = a->ldx; o.ldw = a->ldw; o.ldw2 = a->ldw2; o.ldo = a->ldo; o.ldsx = a->ldsx; o.ldsw = a->ldsw; o.ldsw2 = a->ldsw2; o.ldso = a->ldso;
+    o.M = a->M; o.N = a->N; o.K = a->K; o.out_f32 = a->out_f32;
+    if (o.w2 && (!o.sw2 || !o.so)) return ACV_ERR_SIZE;
+    return ft_run(o, a->flags, a->plan, (int*)const_cast<void*>(a->status), a->sms, (cudaStream_t)const_cast<void*>(a->stream));
 }

@@ -96,9 +96,19 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __rest
 }
 
 // x [T,K] float or bfloat16, rows dense at stride ldx; q [T,K] bytes at stride ldq; s: block_rows 1: [T][groups of K] at stride lds,
-// 128: [blocks of T][groups of K].
-ACV_API int acv_quantize_fp8(const void* x, int dtype, long long ldx, void* q, long long ldq, float* s, long long lds, int T, int K,
-                             int block_rows, int sms, cudaStream_t stream) {
+// 128: [blocks of T][groups of K].  (One record, field for field as kernels/ops.py packs it.)
+struct QuantizeFp8Args {
+    const void *x, *q, *s, *stream;
+    long long ldx, ldq, lds;
+    int dtype, T, K, block_rows, sms;
+};
+ACV_API int acv_quantize_fp8(const QuantizeFp8Args* a) {
+    const void* x = a->x;
+    uint8_t* q = (uint8_t*)const_cast<void*>(a->q);
+    float* s = (float*)const_cast<void*>(a->s);
+    const long long ldx = a->ldx, ldq = a->ldq, lds = a->lds;
+    const int dtype = a->dtype, T = a->T, K = a->K, block_rows = a->block_rows, sms = a->sms;
+    const cudaStream_t stream = (cudaStream_t)const_cast<void*>(a->stream);
     if (T <= 0 || K <= 0) return 0;
     if (dtype != ACV_F32 && dtype != ACV_BF16) return ACV_ERR_DTYPE;
     const int f32 = dtype == ACV_F32;
@@ -108,8 +118,8 @@ ACV_API int acv_quantize_fp8(const void* x, int dtype, long long ldx, void* q, l
         const long long down = ((long long)T + FP8_GROUP - 1) / FP8_GROUP;
         if (down > 65535) return ACV_ERR_SIZE;
         const dim3 grid(G, (unsigned)down);
-        if (vec) acv_launch(PDL_MISC, quantize_blocks_kernel<true>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K);
-        else acv_launch(PDL_MISC, quantize_blocks_kernel<false>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K);
+        if (vec) acv_launch(PDL_MISC, quantize_blocks_kernel<true>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K);
+        else acv_launch(PDL_MISC, quantize_blocks_kernel<false>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K);
         return acv_launch_status();
     }
     if (block_rows != 1) return ACV_ERR_SIZE;
@@ -120,8 +130,8 @@ ACV_API int acv_quantize_fp8(const void* x, int dtype, long long ldx, void* q, l
     const int step_rows = (int)(stride / G), step_groups = (int)(stride % G);
     if ((long long)T + 4ll * (step_rows + 1) > 0x7fffffffll) return ACV_ERR_SIZE;
     if (!vec)
-        acv_launch(PDL_MISC, quantize_rows_kernel<false, 1>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K, G, step_rows, step_groups);
+        acv_launch(PDL_MISC, quantize_rows_kernel<false, 1>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K, G, step_rows, step_groups);
     else
-        acv_launch(PDL_MISC, quantize_rows_kernel<true, 4>, grid, 256, 0, stream, x, f32, ldx, (uint8_t*)q, ldq, s, lds, T, K, G, step_rows, step_groups);
+        acv_launch(PDL_MISC, quantize_rows_kernel<true, 4>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K, G, step_rows, step_groups);
     return acv_launch_status();
 }

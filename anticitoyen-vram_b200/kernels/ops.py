@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import struct
 from ctypes import c_float, c_int, c_void_p
 
 import torch
@@ -146,10 +147,6 @@ def _declare(lib: ctypes.CDLL) -> None:
         "acv_moe_combine": [P, I, I, P, I, P, I, P, P, I, I, I, I, P],
         "acv_glu": [P, I, P, I, I, I, I, F, F, I, I, P],
         "acv_gemm_tc_glu": [P, I, P, I, P, I, I, I, I, F, F, I, P, I, I, I, P],
-        "acv_quantize_fp8": [P, I, LL, P, LL, P, LL, I, I, I, I, P],
-        "acv_add_gated_norms": [P, I, LL, P, I, LL, P, I, LL, P, P, F, F, P, F, P, I, LL, P, LL, I, I, P],
-        "acv_linear_fp8": [P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, I, P, I, P],
-        "acv_linear_fp8_swiglu": [P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, P, LL, I, I, I, I, I, P, I, P],
         "acv_argmax": [P, I, I, I, P, P],
         "acv_apply_penalties": [P, I, I, P, P, P, I, P, P, P, P],
         "acv_sample": [P, I, I, I, P, P, P, P, P, P, P, P, P],
@@ -173,6 +170,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.acv_random_int.restype = c_int
     lib.acv_gemm_tc_test_fault.argtypes = [c_int, c_int]
     lib.acv_gemm_tc_test_fault.restype = None
+    for name in ("acv_quantize_fp8", "acv_add_gated_norms", "acv_linear_fp8"):       # one packed record each
+        getattr(lib, name).argtypes = [ctypes.c_char_p]
+        getattr(lib, name).restype = c_int
     lib.acv_gemm_fp8_test_fault.argtypes = [c_int, c_int]
     lib.acv_gemm_fp8_test_fault.restype = None
 
@@ -2390,56 +2390,72 @@ def fp8_rows(rows: int, columns: int, device) -> tuple[torch.Tensor, torch.Tenso
     return values, torch.empty((rows, (columns + 127) // 128), device=device, dtype=torch.float32)
 
 
-def _one_device(name: str, *tensors) -> int:
-    """The device that all of them lie on."""
-    device = tensors[0].get_device()
-    if device < 0:
-        raise KernelError("acvram_b200 kernels run on a CUDA device only; got a CPU tensor")
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            raise KernelError(f"{name}: the tensors lie on different devices")
-    return device
+# These calls are short, and many of a step: a call's arguments travel as one packed record (fields as the C structs of that name have
+# them; ctypes takes as long for a dozen arguments as the launch itself), the checks read each tensor's shape, type and strides once,
+# and only a call that is refused, or has a column of a single element, goes through the words about it.
+_LINEAR_ARGS = struct.Struct("@10Q8q7i")        # Fp8LinearArgs
+_QUANTIZE_ARGS = struct.Struct("@4Q3q5i")       # QuantizeFp8Args
+_NORMS_ARGS = struct.Struct("@9Q5q6i3f")        # GatedNormsArgs
+_entries: dict = {}
 
 
-def _launch_on(device: int, name: str, entry, *args) -> None:
-    """Launch on that device's current stream, whichever device is current."""
+def _launch_record(device: int, name: str, record: struct.Struct, at: int, *fields) -> None:
+    """Launch the kernel's entry with these fields, the current stream of ``device`` put in as the one at ``at``."""
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = getattr(library(), "acv_" + name)
     if device == torch._C._cuda_getDevice():
-        _check(entry(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+        _check(entry(record.pack(*fields[:at], torch._C._cuda_getCurrentRawStream(device), *fields[at:])), name)
     else:
         with torch.cuda.device(device):
-            _check(entry(*args, torch._C._cuda_getCurrentRawStream(device)), name)
+            _check(entry(record.pack(*fields[:at], torch._C._cuda_getCurrentRawStream(device), *fields[at:])), name)
+
+
+def _sms_of(device: int) -> int:
+    return _sm_counts.get(device) or sm_count(torch.device("cuda", device))
+
+
+def _one_device(name: str, *tensors) -> None:
+    """Raises unless all of them lie on one CUDA device."""
+    devices = {t.get_device() for t in tensors if t is not None}
+    if min(devices) < 0:
+        raise KernelError("acvram_b200 kernels run on a CUDA device only; got a CPU tensor")
+    if len(devices) > 1:
+        raise KernelError(f"{name}: the tensors lie on different devices")
+
+
+def _dense(name: str, what: str, t: torch.Tensor, shape: tuple, dtypes: tuple) -> None:
+    """Raises unless t is a matrix of that shape and one of those types, its rows dense."""
+    if t.dtype not in dtypes or tuple(t.shape) != shape or (t.stride(1) != 1 and shape[1] > 1):
+        raise KernelError(f"{name}: {what} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)} {list(shape)} with dense rows, "
+                          f"got {str(t.dtype).removeprefix('torch.')} {list(t.shape)} strides {t.stride()}")
 
 
 def _fp8_pair(name: str, what: str, values: torch.Tensor, scales: torch.Tensor, rows: int, columns: int, block_rows: int) -> None:
     """Raises unless (values, scales) are a quantised matrix of that size with dense rows."""
-    if values.dtype != FP8 or values.shape != (rows, columns) or (values.stride(1) != 1 and columns > 1):
-        raise KernelError(f"{name}: {what} must be float8_e4m3fn [{rows}, {columns}] with dense rows, got {values.dtype} "
-                          f"{list(values.shape)} strides {values.stride()}")
-    want = (rows if block_rows == 1 else (rows + 127) // 128, (columns + 127) // 128)
-    if scales.dtype != torch.float32 or scales.shape != want or (scales.stride(1) != 1 and want[1] > 1):
-        raise KernelError(f"{name}: the scales of {what} must be float32 {list(want)} with dense rows, got {scales.dtype} "
-                          f"{list(scales.shape)} strides {scales.stride()}")
+    _dense(name, what, values, (rows, columns), (FP8,))
+    _dense(name, "the scales of " + what, scales, (rows if block_rows == 1 else (rows + 127) // 128, (columns + 127) // 128), (torch.float32,))
 
 
 def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
     """(values, scales) of x [R, C] (float32 or bfloat16, dense rows at any stride), in groups of 128 of a row (``block_rows`` 1) or
     in blocks of 128 x 128 (``block_rows`` 128): s = max(largest magnitude / 448, 2^-126), value = e4m3(x * (1 / s)), each step
     rounded once.  A group with a NaN becomes NaN as a whole; one with an infinity gets an infinite scale."""
-    if x.dim() != 2 or block_rows not in (1, 128):
+    shape, dtype, device = x.shape, x.dtype, x.get_device()
+    if len(shape) != 2 or block_rows not in (1, 128):
         raise KernelError("quantize_fp8: a matrix, and block_rows 1 or 128, are wanted")
-    R, C = x.shape
-    if x.stride(1) != 1 and C > 1:
-        raise KernelError("quantize_fp8: the rows of x must be dense")
-    _fp8_pair("quantize_fp8", "the result", values, scales, R, C, block_rows)
-    device = _one_device("quantize_fp8", x, values, scales)
+    R, C = shape
+    xs, vs, ss = x.stride(), values.stride(), scales.stride()
+    if not (dtype in _DT and values.dtype is FP8 and scales.dtype is torch.float32 and values.shape == shape
+            and scales.shape == (R if block_rows == 1 else (R + 127) // 128, (C + 127) // 128) and xs[1] == 1 and vs[1] == 1 and ss[1] == 1
+            and device >= 0 and values.get_device() == device and scales.get_device() == device):
+        _dense("quantize_fp8", "x", x, (R, C), (torch.float32, torch.bfloat16))
+        _fp8_pair("quantize_fp8", "the result", values, scales, R, C, block_rows)
+        _one_device("quantize_fp8", x, values, scales)
     if R and C:
-        _launch_on(device, "quantize_fp8", library().acv_quantize_fp8, x.data_ptr(), dtype_code(x.dtype), x.stride(0), values.data_ptr(),
-                   values.stride(0), scales.data_ptr(), scales.stride(0), R, C, block_rows, sm_count(x.device))
+        _launch_record(device, "quantize_fp8", _QUANTIZE_ARGS, 3, x.data_ptr(), values.data_ptr(), scales.data_ptr(), xs[0], vs[0], ss[0],
+                       _DT[dtype], R, C, block_rows, _sms_of(device))
     return values, scales
-
-
-def _fp8_plan(plan: tuple | None) -> int:
-    return 0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16
 
 
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
@@ -2451,19 +2467,25 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     The weights are read while the kernel in front of this one may still run: they were written long before.  ``plan``: (kind, columns
     of a tile, splits of K) as csrc/gemm_fp8_tc.cu names them, in place of its own choice."""
     T, K = x.shape
-    N = w.shape[0]
-    _fp8_pair("linear_fp8", "x", x, x_scales, T, K, 1)
-    _fp8_pair("linear_fp8", "w", w, w_scales, N, K, 128)
-    if out.shape != (T, N) or (out.stride(1) != 1 and N > 1):
-        raise KernelError(f"linear_fp8: out must be [{T}, {N}] with dense rows, got {list(out.shape)} strides {out.stride()}")
-    device = _one_device("linear_fp8", x, x_scales, w, w_scales, out)
+    N, Kw = w.shape
+    G = (K + 127) // 128
+    xs, xss, ws, wss, outs = x.stride(), x_scales.stride(), w.stride(), w_scales.stride(), out.stride()
+    device = x.get_device()
+    if not (Kw == K and x.dtype is FP8 and w.dtype is FP8 and x_scales.dtype is torch.float32 and w_scales.dtype is torch.float32
+            and out.dtype in _DT and x_scales.shape == (T, G) and w_scales.shape == ((N + 127) // 128, G) and out.shape == (T, N)
+            and xs[1] == 1 and xss[1] == 1 and ws[1] == 1 and wss[1] == 1 and outs[1] == 1 and device >= 0
+            and x_scales.get_device() == device and w.get_device() == device and w_scales.get_device() == device and out.get_device() == device):
+        _fp8_pair("linear_fp8", "x", x, x_scales, T, K, 1)
+        _fp8_pair("linear_fp8", "w", w, w_scales, N, K, 128)
+        _dense("linear_fp8", "out", out, (T, N), (torch.float32, torch.bfloat16))
+        _one_device("linear_fp8", x, x_scales, w, w_scales, out)
     if not T or not N:
         return out
     if not K:
         return out.zero_()
-    _launch_on(device, "linear_fp8", library().acv_linear_fp8, x.data_ptr(), x.stride(0), x_scales.data_ptr(), x_scales.stride(0),
-               w.data_ptr(), w.stride(0), w_scales.data_ptr(), w_scales.stride(0), out.data_ptr(), out.stride(0),
-               1 if dtype_code(out.dtype) == F32 else 0, T, N, K, 1, _fp8_plan(plan), _status_pointer(x), sm_count(x.device))
+    _launch_record(device, "linear_fp8", _LINEAR_ARGS, 9, x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(),
+                   0, 0, 0, _status_at.get(device) or _status_pointer(x) or 0, xs[0], xss[0], ws[0], wss[0], outs[0], 0, 0, 0, T, N, K,
+                   out.dtype is torch.float32, 1, 0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16, _sms_of(device))
     return out
 
 
@@ -2473,20 +2495,31 @@ def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tenso
     """(out, out_scales) = silu(x @ gate^T) * (x @ up^T), quantised in groups of 128 units: what the next ``linear_fp8`` reads.
     Operands as there, gate and up [I, K] each with its own scales.  Unit and quantisation are float, from the float sums."""
     T, K = x.shape
-    I = gate.shape[0]
-    _fp8_pair("linear_fp8_swiglu", "x", x, x_scales, T, K, 1)
-    _fp8_pair("linear_fp8_swiglu", "gate", gate, gate_scales, I, K, 128)
-    _fp8_pair("linear_fp8_swiglu", "up", up, up_scales, I, K, 128)
-    _fp8_pair("linear_fp8_swiglu", "the result", out, out_scales, T, I, 1)
-    device = _one_device("linear_fp8_swiglu", x, x_scales, gate, gate_scales, up, up_scales, out, out_scales)
+    I, Kw = gate.shape
+    G, B = (K + 127) // 128, (I + 127) // 128
+    xs, xss, gs, gss, us, uss = x.stride(), x_scales.stride(), gate.stride(), gate_scales.stride(), up.stride(), up_scales.stride()
+    outs, outss = out.stride(), out_scales.stride()
+    device = x.get_device()
+    if not (Kw == K and x.dtype is FP8 and gate.dtype is FP8 and up.dtype is FP8 and out.dtype is FP8 and x_scales.dtype is torch.float32
+            and gate_scales.dtype is torch.float32 and up_scales.dtype is torch.float32 and out_scales.dtype is torch.float32
+            and up.shape == (I, K) and x_scales.shape == (T, G) and gate_scales.shape == (B, G) and up_scales.shape == (B, G)
+            and out.shape == (T, I) and out_scales.shape == (T, B) and xs[1] == 1 and xss[1] == 1 and gs[1] == 1 and gss[1] == 1
+            and us[1] == 1 and uss[1] == 1 and outs[1] == 1 and outss[1] == 1 and device >= 0 and x_scales.get_device() == device
+            and gate.get_device() == device and gate_scales.get_device() == device and up.get_device() == device
+            and up_scales.get_device() == device and out.get_device() == device and out_scales.get_device() == device):
+        _fp8_pair("linear_fp8_swiglu", "x", x, x_scales, T, K, 1)
+        _fp8_pair("linear_fp8_swiglu", "gate", gate, gate_scales, I, K, 128)
+        _fp8_pair("linear_fp8_swiglu", "up", up, up_scales, I, K, 128)
+        _fp8_pair("linear_fp8_swiglu", "the result", out, out_scales, T, I, 1)
+        _one_device("linear_fp8_swiglu", x, x_scales, gate, gate_scales, up, up_scales, out, out_scales)
     if not T or not I:
         return out, out_scales
     if not K:
         raise KernelError("linear_fp8_swiglu: K is 0")
-    _launch_on(device, "linear_fp8_swiglu", library().acv_linear_fp8_swiglu, x.data_ptr(), x.stride(0), x_scales.data_ptr(),
-               x_scales.stride(0), gate.data_ptr(), gate.stride(0), gate_scales.data_ptr(), gate_scales.stride(0), up.data_ptr(),
-               up.stride(0), up_scales.data_ptr(), up_scales.stride(0), out.data_ptr(), out.stride(0), out_scales.data_ptr(),
-               out_scales.stride(0), T, I, K, 1, _fp8_plan(plan), _status_pointer(x), sm_count(x.device))
+    _launch_record(device, "linear_fp8", _LINEAR_ARGS, 9, x.data_ptr(), x_scales.data_ptr(), gate.data_ptr(), gate_scales.data_ptr(),
+                   out.data_ptr(), up.data_ptr(), up_scales.data_ptr(), out_scales.data_ptr(), _status_at.get(device) or _status_pointer(x) or 0,
+                   xs[0], xss[0], gs[0], gss[0], outs[0], us[0], uss[0], outss[0], T, I, K, 0, 1,
+                   0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16, _sms_of(device))
     return out, out_scales
 
 
@@ -2502,31 +2535,63 @@ def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tens
     x and delta float32 or bfloat16; ``gate`` float32 [H], or [T, H] float32 or bfloat16; weights float32 [H].  out float32 or
     bfloat16, rounded once, or float8_e4m3fn with ``out_scales``: quantised in groups of 128 as ``quantize_fp8`` does.  Matrices
     have dense rows at any stride; H up to 16384.  Sums and both statistics are 32-bit."""
-    T, H = x.shape
-    for t in (x, delta, gate if gate is not None and gate.dim() == 2 else None, out):
-        if t is not None and (t.shape != x.shape or (t.stride(1) != 1 and H > 1)):
-            raise KernelError("add_gated_norms: delta, a gate by tokens and out are of the stream's shape, all with dense rows")
-    vector = gate if gate is not None and gate.dim() != 2 else None
-    for v in (post_weight, weight, vector):
-        if v is not None and (v.dtype != torch.float32 or v.shape != (H,) or (v.stride(0) != 1 and H > 1)):
-            raise KernelError("add_gated_norms: weights and a gate by channels are dense float32 vectors of the stream's width")
-    if delta is None and (gate is not None or post_weight is not None):
-        raise KernelError("add_gated_norms: a gate or a norm behind the part, but no delta")
+    shape, device = x.shape, x.get_device()
+    T, H = shape
+    floats = (torch.float32, torch.bfloat16)
+    name = "add_gated_norms"
+    xs = x.stride()
+    ok = x.dtype in _DT and xs[1] == 1 and device >= 0
+    d_at = d_type = d_ld = g_at = g_type = g_ld = gc_at = w1_at = w2_at = out_at = out_ld = s_at = s_ld = 0
     kind = 3
+    if delta is not None:
+        ds = delta.stride()
+        ok = ok and delta.shape == shape and delta.dtype in _DT and ds[1] == 1 and delta.get_device() == device
+        d_at, d_type, d_ld = delta.data_ptr(), _DT.get(delta.dtype, 0), ds[0]
+    elif gate is not None or post_weight is not None:
+        raise KernelError("add_gated_norms: a gate or a norm behind the part, but no delta")
+    if gate is not None:
+        gs = gate.stride()
+        if len(gs) == 2:
+            ok = ok and gate.shape == shape and gate.dtype in _DT and gs[1] == 1
+            g_at, g_type, g_ld = gate.data_ptr(), _DT.get(gate.dtype, 0), gs[0]
+        else:
+            ok = ok and gate.dtype is torch.float32 and gate.shape == (H,) and gs[0] == 1
+            gc_at = gate.data_ptr()
+        ok = ok and gate.get_device() == device
+    if post_weight is not None:
+        ok = ok and post_weight.dtype is torch.float32 and post_weight.shape == (H,) and post_weight.stride(0) == 1 and post_weight.get_device() == device
+        w1_at = post_weight.data_ptr()
     if out is not None:
+        if weight is None:
+            raise KernelError("add_gated_norms: a result wants a weight")
         kind = _NORM_OUT.get(out.dtype, 3)
-        if kind == 3 or weight is None or (kind == 2) != (out_scales is not None):
-            raise KernelError("add_gated_norms: out is float32, bfloat16, or float8_e4m3fn with out_scales, and wants a weight")
-        if kind == 2:
-            _fp8_pair("add_gated_norms", "out", out, out_scales, T, H, 1)
+        outs = out.stride()
+        ok = ok and kind < 3 and out.shape == shape and outs[1] == 1 and out.get_device() == device and (kind == 2) == (out_scales is not None) \
+            and weight.dtype is torch.float32 and weight.shape == (H,) and weight.stride(0) == 1 and weight.get_device() == device
+        w2_at, out_at, out_ld = weight.data_ptr(), out.data_ptr(), outs[0]
+        if out_scales is not None:
+            ss = out_scales.stride()
+            ok = ok and out_scales.dtype is torch.float32 and out_scales.shape == (T, (H + 127) // 128) and ss[1] == 1 and out_scales.get_device() == device
+            s_at, s_ld = out_scales.data_ptr(), ss[0]
     elif out_scales is not None:
         raise KernelError("add_gated_norms: scales without a result")
-    device = _one_device("add_gated_norms", x, delta, gate, post_weight, weight, out, out_scales)
+    if not ok:
+        _dense(name, "x", x, (T, H), floats)
+        if delta is not None:
+            _dense(name, "delta", delta, (T, H), floats)
+        if g_at:
+            _dense(name, "a gate by tokens", gate, (T, H), floats)
+        for what, v in (("post_weight", post_weight), ("weight", weight if out is not None else None), ("a gate by channels", gate if gc_at else None)):
+            if v is not None and (v.dtype != torch.float32 or tuple(v.shape) != (H,) or (v.stride(0) != 1 and H > 1)):
+                raise KernelError(f"{name}: {what} must be a dense float32 vector of {H}, got {v.dtype} {list(v.shape)} strides {v.stride()}")
+        if out is not None:
+            if (out.dtype == FP8) != (out_scales is not None):
+                raise KernelError(f"{name}: out_scales go with a result of float8_e4m3fn, and only with one")
+            _dense(name, "out", out, (T, H), tuple(_NORM_OUT))
+            if out_scales is not None:
+                _fp8_pair(name, "out", out, out_scales, T, H, 1)
+        _one_device(name, x, delta, gate, post_weight, weight if out is not None else None, out, out_scales)
     if T and H:
-        rows = gate if vector is None else None
-        _launch_on(device, "add_gated_norms", library().acv_add_gated_norms, x.data_ptr(), dtype_code(x.dtype), x.stride(0), _p(delta),
-                   0 if delta is None else dtype_code(delta.dtype), 0 if delta is None else delta.stride(0), _p(rows),
-                   0 if rows is None else dtype_code(rows.dtype), 0 if rows is None else rows.stride(0), _p(vector), _p(post_weight),
-                   post_eps, residual_scale, _p(weight), eps, _p(out), kind if kind < 3 else 0, 0 if out is None else out.stride(0),
-                   _p(out_scales), 0 if out_scales is None else out_scales.stride(0), T, H)
+        _launch_record(device, name, _NORMS_ARGS, 8, x.data_ptr(), d_at, g_at, gc_at, w1_at, w2_at, out_at, s_at, xs[0], d_ld, g_ld, out_ld,
+                       s_ld, _DT[x.dtype], d_type, g_type, kind, T, H, residual_scale, post_eps, eps)
     return out
