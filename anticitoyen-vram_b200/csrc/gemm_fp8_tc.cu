@@ -20,72 +20,7 @@
 // Warps: 0 loads, 1 issues the products, from 2 on they are the epilogue, each a quarter of the lanes.  Every wait on an mbarrier is
 // bounded; when one runs out the kernel records where in `status`, all roles leave their loops, the loads in flight are waited for
 // (with a limit), tensor memory is freed and the kernel returns.
-#include "fp8.cuh"
-#include "tc_ptx.cuh"
-#include "tensor_map.h"
-#include "gemm_fp8.h"
-
-#define FT_ROWS 128                         // rows of an operand tile = bytes of a k-block's row
-#define FT_TILE (FT_ROWS * FT_ROWS)         // bytes of an operand tile of 128 rows
-
-struct Fp8TcParams {
-    int M, N, n_kb;                         // N: features, or units of the gated form
-    const float *sx, *sw, *sw2;             // sw2: the up rows' scales of the gated form
-    long long ldsx, ldsw, ldsw2, ldo, ldso;
-    void* out;
-    float* so;
-    int out_f32, out_vec, sx_vec;           // _vec: rows of out take 16-byte stores, those of sx 16-byte loads
-    int tiles_m, tiles_n, group, stages, splits, kb_per_split, early_w;
-    int* status;
-    unsigned int wait_limit;                // of polls; less and a k-block whose loads are left out (skip_kb >= 0) in the test of the waits only
-    int skip_kb;
-};
-
-__device__ __forceinline__ uint32_t ft_idesc(int n, int m) {        // float accumulator, e4m3 operands (type 0), both K-major
-    return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-// One lane of a converged warp.  The issuing warp runs its loop as a whole and lets this lane issue: what the products need is then
-// known to be the warp's and is kept in uniform registers.  (A loop run by one lane alone moved every descriptor there first: 600
-// cycles a k-block, where the tensor core needs 512 for the largest.)
-__device__ __forceinline__ bool ft_elect() {
-    uint32_t yes;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
-    return yes != 0;
-}
-__device__ __forceinline__ int ft_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
-template <bool PAIR>
-__device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    if (PAIR)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                     ::"r"(tmem_d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate) : "memory");
-}
-// the registers of a load are what its wait hands over: nothing that reads them moves in front of it
-__device__ __forceinline__ void ft_wait_ld(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
-}
-__device__ __forceinline__ void ft_fma2(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t scale) {
-    asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(scale));
-}
-__device__ __forceinline__ uint64_t ft_both(float v) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(v)));
-    return r;
-}
-__device__ __forceinline__ uint64_t ft_pair(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(lo)), "r"(__float_as_uint(hi)));
-    return r;
-}
-__device__ __forceinline__ float2 ft_floats(uint64_t v) {
-    uint32_t lo, hi;
-    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
+#include "fp8_tc.cuh"
 
 // sums[0 .. 8 PIECES) += scales * 16 PIECES columns of this lane's row, the first half of them from `first`, the others from `second`;
 // a piece of sixteen is on its way while the one before is added
@@ -185,26 +120,6 @@ __device__ __forceinline__ void ft_tile_of(int tile, int tiles_m, int tiles_n, i
     tb = r / rows;
     ta = g * group + (r - tb * rows);
 }
-// After a wait that ran out: the loads that are still under way write into this CTA's shared memory, so their stages are waited for
-// (each by the parity of the last of `asked` k-blocks that went into it), with a limit.
-__device__ __forceinline__ void ft_drain(uint32_t full0, int stages, int asked, unsigned int limit) {
-    for (int s = 0; s < stages && s < asked; ++s) {
-        const int last = (asked - 1 - s) / stages;
-        for (unsigned int i = 0; i < limit; ++i)
-            if (mbar_try_wait(full0 + 8 * s, last & 1)) break;
-    }
-}
-
-// a wait by a whole warp: true for all of its lanes where it ran out for one
-__device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Fp8TcParams& p, int code = 4) {
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit));
-    if (!ok && (threadIdx.x & 31) == 0) {
-        *abort_flag = 1;
-        atomicExch(p.status, code);
-    }
-    return !ok;
-}
-
 // ----------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256
 #define FP_STAGE (2 * FT_TILE)              // a CTA's share of a k-block: 128 rows of tokens, 128 of weights
 #define FP_MAX_STAGES 6
@@ -427,12 +342,6 @@ struct Fp8TileShape {
     static constexpr int smem(int stages) { return 1024 + (stages * STAGE > SUMS ? stages * STAGE : SUMS) + 256; }
 };
 
-__device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-
 // GATED: BN is 256, the columns are 128 units' gate rows and their up rows, and a row of the result is a whole group.
 template <int BN, bool GATED>
 __global__ void __launch_bounds__(Fp8TileShape<BN>::THREADS, 1)
@@ -566,70 +475,8 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     tc_fence_before();
     if (p.splits > 1) cluster_sync_all();
     else __syncthreads();
-    // The rows of the tile are dealt out to the cluster's CTAs and their warps; a lane takes four neighbouring columns at a time.
-    const int rows = min(FT_ROWS, p.M - row_here);
-    const uint32_t own = tiles_addr;
-    if (!abort_s) {
-#pragma unroll 1
-        for (int r = split + p.splits * warp; r < rows; r += p.splits * (S::THREADS / 32)) {
-            auto sum4 = [&](int c) {
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                const uint32_t at = own + (uint32_t)(r * S::LD + c) * 4;
-                for (int q = 0; q < p.splits; ++q) {
-                    const float4 o = ft_cluster_read4(cluster_map(at, q));
-                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-                }
-                return v;
-            };
-            const size_t row = (size_t)(row_here + r);
-            if (GATED) {
-                const float4 g = sum4(4 * lane), u = sum4(FT_ROWS + 4 * lane);
-                const float h[4] = {silu_f32<float>(g.x) * u.x, silu_f32<float>(g.y) * u.y, silu_f32<float>(g.z) * u.z, silu_f32<float>(g.w) * u.w};
-                uint32_t m = max(max(fp8_magnitude(h[0]), fp8_magnitude(h[1])), max(fp8_magnitude(h[2]), fp8_magnitude(h[3])));
-                m = __reduce_max_sync(0xffffffffu, m);
-                const Fp8Scale k = fp8_scale(m);
-                const uint32_t w = fp8_pack4(h[0], h[1], h[2], h[3], k.r);
-                if (lane == 0) p.so[row * p.ldso + tb] = k.s;
-                const int u0 = tb * FT_ROWS + 4 * lane;
-                uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + row * p.ldo + u0;
-                if (p.out_vec && u0 + 4 <= p.N) {
-                    *reinterpret_cast<uint32_t*>(o) = w;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (u0 + c < p.N) o[c] = (uint8_t)(w >> (8 * c));
-                }
-            } else {
-#pragma unroll
-                for (int c = 4 * lane; c < BN; c += 128) {
-                    const float4 v = sum4(c);
-                    const int n = tb * BN + c;
-                    if (n >= p.N) continue;
-                    if (p.out_f32) {
-                        float* o = reinterpret_cast<float*>(p.out) + row * p.ldo + n;
-                        if (p.out_vec && n + 4 <= p.N) {
-                            *reinterpret_cast<float4*>(o) = v;
-                        } else {
-                            o[0] = v.x;
-                            if (n + 1 < p.N) o[1] = v.y;
-                            if (n + 2 < p.N) o[2] = v.z;
-                            if (n + 3 < p.N) o[3] = v.w;
-                        }
-                    } else {
-                        bf16* o = reinterpret_cast<bf16*>(p.out) + row * p.ldo + n;
-                        if (p.out_vec && n + 4 <= p.N) {
-                            *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
-                        } else {
-                            o[0] = __float2bfloat16_rn(v.x);
-                            if (n + 1 < p.N) o[1] = __float2bfloat16_rn(v.y);
-                            if (n + 2 < p.N) o[2] = __float2bfloat16_rn(v.z);
-                            if (n + 3 < p.N) o[3] = __float2bfloat16_rn(v.w);
-                        }
-                    }
-                }
-            }
-        }
-    }
+    if (!abort_s)
+        ft_emit<BN, GATED, 1, 2>(p, tiles_addr, S::LD, split + p.splits * warp, p.splits * (S::THREADS / 32), min(FT_ROWS, p.M - row_here), row_here, tb);
     // (the peers may still read this CTA's sums)
     if (p.splits > 1) cluster_sync_all();
     if (warp == 1) {
@@ -639,20 +486,6 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 }
 
 // ----------------------------------------------------------------------------- host side
-// tensor map of a matrix of bytes [rows, K] with row stride ld: box = 128 x box_rows, 128-byte swizzle
-static int ft_map(CUtensorMap* map, const void* base, int rows, int K, long long ld, int box_rows) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return ACV_ERR_SIZE;
-    const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)ld};
-    const cuuint32_t box[2] = {FT_ROWS, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : ACV_ERR_ALIGN;
-}
-
 // Test of the bounded waits, without a fault: the next product launched from this process polls each mbarrier at most `wait_limit`
 // times and its producer leaves out the loads of k-block `skip_kb` (the codes are those of acv_gemm_tc_test_fault; the output of that
 // launch is unspecified).
@@ -726,7 +559,8 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
     return acv_launch_status();
 }
 
-// How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs.
+// How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs, 4 weight
+// rows on the tensor core's rows, bn tokens to a tile, K over `splits` CTAs (gemm_fp8_narrow.cu).
 struct Fp8Plan { int kind, bn, splits; };
 static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
     if (M <= 16) return {1, 0, 1};
@@ -756,12 +590,15 @@ static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cud
     p.skip_kb = g_test_skip_kb;
     g_test_wait_limit = 0; g_test_skip_kb = -1;
     CUtensorMap mx, mw, mw2;
-    if (const int rc = ft_map(&mx, o.x, o.M, o.K, o.ldx, FT_ROWS)) return rc;
-    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 3 || gated ? FT_ROWS : how.bn)) return rc;
+    if (how.kind == 4 && how.bn != 16 && how.bn != 32 && how.bn != 64) return ACV_ERR_SIZE;
+    if (how.kind == 2 && how.bn != 64 && how.bn != 128 && how.bn != 256) return ACV_ERR_SIZE;
+    if (const int rc = ft_map(&mx, o.x, o.M, o.K, o.ldx, how.kind == 4 ? how.bn : FT_ROWS)) return rc;
+    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 2 && !gated ? how.bn : how.kind == 4 && gated ? 64 : FT_ROWS)) return rc;
     mw2 = mw;
     if (gated)
-        if (const int rc = ft_map(&mw2, o.w2, o.N, o.K, o.ldw2, FT_ROWS)) return rc;
+        if (const int rc = ft_map(&mw2, o.w2, o.N, o.K, o.ldw2, how.kind == 4 ? 64 : FT_ROWS)) return rc;
     if (how.kind == 3) return gated ? ft_launch_pair<true>(mx, mw, mw2, p, sms, stream) : ft_launch_pair<false>(mx, mw, mw2, p, sms, stream);
+    if (how.kind == 4) return acv_fp8_narrow(mx, mw, mw2, p, gated, how.bn, how.splits, sms, stream);
     if (how.kind != 2) return ACV_ERR_SIZE;
     if (gated) return how.bn == 256 ? ft_launch_tile<256, true>(mx, mw, mw2, p, how.splits, stream) : ACV_ERR_SIZE;
     switch (how.bn) {

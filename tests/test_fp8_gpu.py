@@ -134,7 +134,8 @@ def test_product_of_other_sizes(T, N, K):
     check_product(T, N, K, F32, T + N + K, (1, 2, 3))
 
 
-@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 64, 1), (2, 64, 3), (2, 128, 1), (2, 128, 2), (2, 128, 8), (3, 256, 1)])
+@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 64, 1), (2, 64, 3), (2, 128, 1), (2, 128, 2), (2, 128, 8), (3, 256, 1),
+                                  (4, 16, 1), (4, 16, 8), (4, 32, 2), (4, 64, 1), (4, 64, 3)])
 @pytest.mark.parametrize("T,N,K,out_dtype", [(1, 128, 128, F32), (5, 300, 400, BF), (140, 130, 1100, F32), (300, 700, 2048, BF), (513, 257, 1296, F32)])
 def test_product_by_every_plan(T, N, K, out_dtype, plan):
     check_product(T, N, K, out_dtype, T + 3, plan=plan)
@@ -203,19 +204,20 @@ def test_gated_product_of_other_sizes(T, I, K):
     check_gated(T, I, K, T + I + K)
 
 
-@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 256, 1), (2, 256, 2), (2, 256, 5), (3, 256, 1)])
+@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 256, 1), (2, 256, 2), (2, 256, 5), (3, 256, 1), (4, 16, 1), (4, 16, 3), (4, 32, 2), (4, 64, 1),
+                                  (4, 64, 4)])
 @pytest.mark.parametrize("T,I,K", [(1, 128, 128), (5, 300, 400), (140, 130, 1100), (300, 700, 2048), (513, 257, 1296)])
 def test_gated_product_by_every_plan(T, I, K, plan):
     check_gated(T, I, K, T + 3, plan=plan)
 
 
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("kind", [2, 3])
+@pytest.mark.parametrize("kind", [2, 3, 4])
 def test_a_wait_that_runs_out_is_reported(kind, gated):
     """A product whose producer leaves out a k-block gives up after a few polls, says so in the status word, and the next one runs."""
     x, xs = quantized(200, 1024, 1, 1)
     w, ws = quantized(300, 1024, 2, 128)
-    plan = (kind, 256 if gated or kind == 3 else 128, 1)
+    plan = (kind, 32 if kind == 4 else 256 if gated or kind == 3 else 128, 1)
 
     def run():
         if gated:
