@@ -201,6 +201,6 @@ static inline int ft_map(CUtensorMap* map, const void* base, int rows, int K, lo
 }
 
 
-// gemm_fp8_narrow.cu: tokens on the columns, `bt` of them (16, 32, 64) to a tile, K over `splits` CTAs
+// gemm_fp8_narrow.cu: tokens on the columns, `bt` of them (16 or 32) to a tile, K over `splits` CTAs
 int acv_fp8_narrow(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mw2, Fp8TcParams& p, bool gated, int bt, int splits,
                    int sms, cudaStream_t stream);

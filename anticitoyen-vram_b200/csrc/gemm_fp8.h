@@ -12,4 +12,4 @@ struct Fp8Operands {
     int M, N, K, out_f32;
 };
 
-int acv_fp8_rows(const Fp8Operands& o, int flags, int sms, cudaStream_t stream);
+int acv_fp8_rows(const Fp8Operands& o, int flags, cudaStream_t stream);

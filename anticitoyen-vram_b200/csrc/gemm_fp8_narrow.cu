@@ -13,7 +13,7 @@
 template <int BT>
 struct Fp8NarrowShape {
     static constexpr int STAGE = FT_TILE + BT * FT_ROWS;
-    static constexpr int RESIDENT = BT == 64 ? 2 : 3;                       // CTAs to an SM at most
+    static constexpr int RESIDENT = 3;                                      // CTAs to an SM at most
     static constexpr int SLOTS = 4;                                         // partial results in tensor memory
     static constexpr int TMEM = SLOTS * BT;
     // registers of a thread: they are handed out for warps rounded up to four
@@ -184,7 +184,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     if (size > 1) cluster_sync_all();
     else __syncthreads();
     if (!abort_s)
-        ft_emit<FT_ROWS, GATED, HALVES, BT == 64 ? 2 : 1>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
+        ft_emit<FT_ROWS, GATED, HALVES, 1>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
     // (the peers may still read this CTA's sums)
     if (size > 1) cluster_sync_all();
     if (warp == 1) {
@@ -204,11 +204,12 @@ static int fn_launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtenso
     p.kb_per_split = (p.n_kb + splits - 1) / splits;
     p.splits = (p.n_kb + p.kb_per_split - 1) / p.kb_per_split;
     const int size = p.splits * HALVES;
-    const long long ctas = (long long)p.tiles_m * p.tiles_n * size;
+    const long long clusters = (long long)p.tiles_m * p.tiles_n, ctas = clusters * size;
     if (ctas > 0x7fffffff) return ACV_ERR_SIZE;
-    // as many stages as the shared memory of an SM gives each of the CTAs that come to it
+    // as many stages as the shared memory of an SM gives each of the CTAs that come to it (by the clusters that fit with one CTA to an SM)
     const int fixed = 1024 + 256 + (p.kb_per_split * HALVES * (BT + 1) * 4 + 127) / 128 * 128;
-    const int here = ctas <= sms ? 1 : ctas <= 2ll * sms ? 2 : S::RESIDENT, budget = 227 * 1024 / here - 1024;
+    const long long fit = (long long)ACV_CLUSTERS_AT_ONCE[size] * sms / 148 + 1;
+    const int here = clusters < fit ? 1 : clusters < 2 * fit - 1 ? 2 : S::RESIDENT, budget = 227 * 1024 / here - 1024;
     if (fixed + S::SUMS > 225 * 1024 || fixed + 2 * S::STAGE > 225 * 1024) return ACV_ERR_SIZE;
     p.stages = (budget - fixed) / S::STAGE;
     p.stages = p.stages < 2 ? 2 : p.stages > 10 ? 10 : p.stages;            // (28 barriers at most in their 256 bytes)
@@ -225,7 +226,6 @@ int acv_fp8_narrow(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorM
     switch (bt) {
         case 16: return gated ? fn_launch<16, true>(mx, mw, mw2, p, splits, sms, stream) : fn_launch<16, false>(mx, mw, mw2, p, splits, sms, stream);
         case 32: return gated ? fn_launch<32, true>(mx, mw, mw2, p, splits, sms, stream) : fn_launch<32, false>(mx, mw, mw2, p, splits, sms, stream);
-        case 64: return gated ? fn_launch<64, true>(mx, mw, mw2, p, splits, sms, stream) : fn_launch<64, false>(mx, mw, mw2, p, splits, sms, stream);
         default: return ACV_ERR_SIZE;
     }
 }

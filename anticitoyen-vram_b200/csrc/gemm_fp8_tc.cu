@@ -13,9 +13,10 @@
 // the CTAs of a cluster, whose sums meet through its shared memory, in rank order, so the result does not depend on timing.
 //
 // What bounds the many-token form beside the tensor core is that hand-over, once for each k-block: from the products' end until the
-// epilogue warps of both CTAs have fetched the partial tile and the issuing thread knows it.  With two partial tiles of 256 columns
-// the tensor core waited for it (4096 x 4096 x 12288 in 211 us, and in as many without any fetch or sum; 155 us with nobody to wait
-// for); with four of 128 columns three others are under way meanwhile.
+// epilogue warps of both CTAs have fetched the partial tile (some 500 cycles, the bandwidth of tensor memory) and the issuing warp has
+// learnt it (as many), with two partial tiles for 512 cycles of tensor core each.  4096 x 4096 x 12288: 204 us; 155 us with nobody to wait for.
+// Finer partial tiles, more epilogue warps or registers taken from the idle warps did not shorten it (four tiles of 128 columns 238 us,
+// sixteen warps 310).
 //
 // Warps: 0 loads, 1 issues the products, from 2 on they are the epilogue, each a quarter of the lanes.  Every wait on an mbarrier is
 // bounded; when one runs out the kernel records where in `status`, all roles leave their loops, the loads in flight are waited for
@@ -336,8 +337,8 @@ struct Fp8TileShape {
     static constexpr int TMEM = SLOTS * BN;
     static constexpr int LD = BN + 4;                               // floats of a row of the summed tile: sixteen-byte stores of eight rows meet no bank twice
     static constexpr int SUMS = FT_ROWS * LD * 4;
-    static constexpr int COLS = BN == 256 ? 128 : 64;               // of an epilogue thread
-    static constexpr int WARPS = 4 * BN / COLS;                     // of the epilogue
+    static constexpr int COLS = BN / 2;                             // of an epilogue thread
+    static constexpr int WARPS = 8;                                 // of the epilogue
     static constexpr int THREADS = 64 + 32 * WARPS;
     static constexpr int smem(int stages) { return 1024 + (stages * STAGE > SUMS ? stages * STAGE : SUMS) + 256; }
 };
@@ -561,15 +562,35 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
 
 // How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs, 4 weight
 // rows on the tensor core's rows, bn tokens to a tile, K over `splits` CTAs (gemm_fp8_narrow.cu).
+//
+// Up to 16 tokens whose weights are one round of blocks of 32 rows stream (microseconds, streaming and the best of kind 4: 8 tokens
+// 4096 x 4096 4.2, 5.4; 6144 x 4096 7.6, 5.8; 4096 x 12288 11.6, 11.2; 16 tokens 4096 x 2560 4.6, 4.9; 1024 x 4096 5.4, 4.1).
+// Up to 32 tokens, and beyond: kind 4 and kind 2, 32 tokens 6144 x 4096 7.2 and 12.7, 64 tokens 6144 x 4096 11.2 and 9.9,
+// 4096 x 12288 15.9 and 14.0, 5120 x 17408 20.8 and 20.8.
+//   Splits of K are what fits the SMs at once in clusters, two CTAs of kind 4 to an SM (three of the gated form, whose cluster holds two
+// halves of a group), one of kind 2, and at least four k-blocks to each: 16 tokens 6144 x 4096 in 2, 4, 6 splits 7.9, 6.1, 9.8; 4096 x 1024
+// in 1, 2, 4: 4.3, 3.8, 4.2; 12288 units, K 4096, in 1, 2, 3: 21.0, 19.2, 24.8; kind 2, 65 tokens 4096 x 12288 in 2, 3, 4, 6: 19.5, 15.9,
+// 14.0, 23.3.
+//   Pairs of CTAs and tiles of 128 rows both come in rounds over the SMs, and a round of pairs takes 1.3 of a round of tiles of 128 x 128,
+// 0.83 of one of gated tiles of 128 x 256 (K 4096: 16.2 us, 21; 37.5, 31.2): 512 tokens 4096 x 4096 16.2 and 19.8, 6144 x 4096 32.1 and 22.5,
+// 384 tokens of 12288 units 76 and 93, 512 of them 113 and 94.
 struct Fp8Plan { int kind, bn, splits; };
 static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
-    if (M <= 16) return {1, 0, 1};
-    const int n_kb = (K + FT_ROWS - 1) / FT_ROWS, tm = (M + FT_ROWS - 1) / FT_ROWS;
-    const int bn = gated ? 256 : 128, tiles = tm * ((N + FT_ROWS - 1) / FT_ROWS);
-    if (tiles > sms) return {3, 256, 1};
+    const long long n_kb = (K + FT_ROWS - 1) / FT_ROWS, wide = (N + FT_ROWS - 1) / FT_ROWS, deep = (M + FT_ROWS - 1) / FT_ROWS;
+    auto fit = [&](int size) { return (long long)ACV_CLUSTERS_AT_ONCE[size] * sms / 148; };
+    if (!gated && M <= 16 && N <= 32ll * sms && K <= (M <= 8 ? 8192 : 2560)) return {1, 0, 1};
     int splits = 1;
-    while (splits < 8 && splits < n_kb && tiles <= ACV_CLUSTERS_AT_ONCE[splits + 1]) ++splits;
-    return {2, bn, splits};
+    if (M <= 32) {
+        if (gated) splits = wide <= 3 * fit(4) && n_kb >= 4 ? 2 : 1;
+        else
+            while (splits < 8 && wide <= 2 * fit(splits + 1) && n_kb >= 4 * (splits + 1)) ++splits;
+        return {4, M <= 16 ? 16 : 32, splits};
+    }
+    const long long tiles = deep * wide, pairs = (deep + 1) / 2 * (gated ? wide : (wide + 1) / 2);
+    const long long tile_rounds = (tiles + sms - 1) / sms, pair_rounds = (pairs + sms / 2 - 1) / (sms / 2);
+    if ((double)pair_rounds * (gated ? 0.83 : 1.3) < (double)tile_rounds) return {3, 256, 1};
+    while (splits < 8 && tiles <= fit(splits + 1) && n_kb >= 4 * (splits + 1)) ++splits;
+    return {2, gated ? 256 : 128, splits};
 }
 
 static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cudaStream_t stream) {
@@ -578,7 +599,7 @@ static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cud
     if (o.K <= 0) return ACV_ERR_SIZE;
     if (((uintptr_t)o.x | (uintptr_t)o.w | (uintptr_t)o.w2) % 16 || (o.ldx | o.ldw | o.ldw2) % 16) return ACV_ERR_ALIGN;
     const Fp8Plan how = plan ? Fp8Plan{plan & 15, (plan >> 4) & 0xfff, plan >> 16} : ft_plan(o.M, o.N, o.K, gated, sms);
-    if (how.kind == 1) return acv_fp8_rows(o, flags, sms, stream);
+    if (how.kind == 1) return acv_fp8_rows(o, flags, stream);
     if (!status) return ACV_ERR_SCRATCH;
     Fp8TcParams p = {};
     p.M = o.M; p.N = o.N; p.n_kb = (o.K + FT_ROWS - 1) / FT_ROWS;
@@ -590,22 +611,17 @@ static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cud
     p.skip_kb = g_test_skip_kb;
     g_test_wait_limit = 0; g_test_skip_kb = -1;
     CUtensorMap mx, mw, mw2;
-    if (how.kind == 4 && how.bn != 16 && how.bn != 32 && how.bn != 64) return ACV_ERR_SIZE;
-    if (how.kind == 2 && how.bn != 64 && how.bn != 128 && how.bn != 256) return ACV_ERR_SIZE;
+    if (how.kind == 4 && how.bn != 16 && how.bn != 32) return ACV_ERR_SIZE;
+    if (how.kind == 2 && how.bn != (gated ? 256 : 128)) return ACV_ERR_SIZE;
     if (const int rc = ft_map(&mx, o.x, o.M, o.K, o.ldx, how.kind == 4 ? how.bn : FT_ROWS)) return rc;
-    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 2 && !gated ? how.bn : how.kind == 4 && gated ? 64 : FT_ROWS)) return rc;
+    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 4 && gated ? 64 : FT_ROWS)) return rc;
     mw2 = mw;
     if (gated)
         if (const int rc = ft_map(&mw2, o.w2, o.N, o.K, o.ldw2, how.kind == 4 ? 64 : FT_ROWS)) return rc;
     if (how.kind == 3) return gated ? ft_launch_pair<true>(mx, mw, mw2, p, sms, stream) : ft_launch_pair<false>(mx, mw, mw2, p, sms, stream);
     if (how.kind == 4) return acv_fp8_narrow(mx, mw, mw2, p, gated, how.bn, how.splits, sms, stream);
     if (how.kind != 2) return ACV_ERR_SIZE;
-    if (gated) return how.bn == 256 ? ft_launch_tile<256, true>(mx, mw, mw2, p, how.splits, stream) : ACV_ERR_SIZE;
-    switch (how.bn) {
-        case 64: return ft_launch_tile<64, false>(mx, mw, mw2, p, how.splits, stream);
-        case 128: return ft_launch_tile<128, false>(mx, mw, mw2, p, how.splits, stream);
-        default: return ACV_ERR_SIZE;
-    }
+    return gated ? ft_launch_tile<256, true>(mx, mw, mw2, p, how.splits, stream) : ft_launch_tile<128, false>(mx, mw, mw2, p, how.splits, stream);
 }
 
 // A call's arguments as one record (a caller through a foreign-function interface pays for each argument by itself), field for field as
