@@ -67,6 +67,16 @@ __device__ __forceinline__ void load8_ragged(const void* row, int f32, int at, i
     for (int i = 0; i < 8; ++i)
         v[i] = at + i >= n ? 0.f : f32 ? reinterpret_cast<const float*>(row)[at + i] : __bfloat162float(reinterpret_cast<const bf16*>(row)[at + i]);
 }
+__device__ __forceinline__ Raw8 raw8_load_ragged(const void* row, int f32, int at, int n) {
+    uint32_t w[8] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (at + i < n) {
+            if (f32) w[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
+            else w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[at + i] << (16 * (i & 1));
+        }
+    return {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
+}
 __device__ __forceinline__ void store8(void* row, int f32, int at, const float (&v)[8]) {
     if (f32) {
         float4* p = reinterpret_cast<float4*>(reinterpret_cast<float*>(row) + at);
@@ -106,6 +116,18 @@ __device__ __forceinline__ uint32_t magnitude8(const float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, fp8_magnitude(v[i]));
     return m;
+}
+// the same of eight elements as they came from memory: bfloat16 magnitudes are ordered as their bits are, two at a time
+__device__ __forceinline__ uint32_t magnitude8(const Raw8& r, int f32) {
+    const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w}, b[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+    if (f32) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = max(m, max(a[i] & 0x7fffffffu, b[i] & 0x7fffffffu));
+        return m;
+    }
+    const uint32_t m = __vmaxu2(__vmaxu2(a[0] & 0x7fff7fffu, a[1] & 0x7fff7fffu), __vmaxu2(a[2] & 0x7fff7fffu, a[3] & 0x7fff7fffu));
+    return max(m << 16, m & 0xffff0000u);
 }
 // the largest over the sixteen lanes that hold a group of 128
 __device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {

@@ -19,7 +19,7 @@ struct GnParams {
     float* s;
     long long ldx, ldd, ldg, ldo, lds;
     int H, x_f32, d_f32, g_f32, out_kind;       // out_kind: 0 float, 1 bfloat16, 2 e4m3, 3 none
-    float c, e1, e2;
+    float c, e1, e2, inv_h;
 };
 
 template <bool VEC>
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
                 }
             }
             ss = block_sum(ss, red);
-            r = 1.f / sqrtf(ss / (float)H + p.e1);
+            r = rsqrtf(fmaf(ss, p.inv_h, p.e1));
         }
 #pragma unroll
         for (int i = 0; i < C; ++i) {
@@ -130,35 +130,47 @@ __global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
             for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
         }
     ss = block_sum(ss, red);
-    const float r = 1.f / sqrtf(ss / (float)H + p.e2);
+    const float r = rsqrtf(fmaf(ss, p.inv_h, p.e2));
     char* o = reinterpret_cast<char*>(p.out) + row * p.ldo * (p.out_kind == 0 ? 4 : p.out_kind == 1 ? 2 : 1);
+    uint32_t own = 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
         const int at = (threadIdx.x + i * blockDim.x) * 8;
         const bool in = at < H;
         if (C > 1 && in) gn_load<VEC>(p.w2, 1, at, H, w2);
-        float h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = (VEC ? in : at + e < H) ? x[i][e] * r * w2[e] : 0.f;      // (zeros behind the row's end)
-        if (p.out_kind == 2) {
-            const Fp8Scale k = fp8_scale(half_warp_max(magnitude8(h)));      // (whole warps pass here)
-            if (in) {
-                store_q8<VEC>(reinterpret_cast<uint8_t*>(o), at, H, h, k.r);
-                if ((threadIdx.x & 15) == 0) p.s[row * p.lds + at / FP8_GROUP] = k.s;
-            }
+        for (int e = 0; e < 8; ++e) x[i][e] = (VEC ? in : at + e < H) ? x[i][e] * r * w2[e] : 0.f;      // (zeros behind the row's end)
+        if (p.out_kind == 2) {          // (whole warps pass here)
+            const uint32_t m = half_warp_max(magnitude8(x[i]));
+            if ((int)(threadIdx.x % C) == i) own = m;
         } else if (in) {
-            if (VEC) store8(o, p.out_kind == 0, at, h);
-            else store8_ragged(o, p.out_kind == 0, at, H, h);
+            if (VEC) store8(o, p.out_kind == 0, at, x[i]);
+            else store8_ragged(o, p.out_kind == 0, at, H, x[i]);
         }
+    }
+    if (p.out_kind != 2) return;
+    // the scales of a half-warp's C groups, made side by side by its lanes
+    const Fp8Scale mine = fp8_scale(own);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int at = (threadIdx.x + i * blockDim.x) * 8;
+        const float k = __shfl_sync(0xffffffffu, mine.r, i, 16);
+        if (at < H) store_q8<VEC>(reinterpret_cast<uint8_t*>(o), at, H, x[i], k);
+        const int group = (int)((threadIdx.x & ~15u) + i * blockDim.x) / 16;
+        if ((int)(threadIdx.x & 15) == i && group * FP8_GROUP < H) p.s[row * p.lds + group] = mine.s;
     }
 }
 
+// Pieces of eight elements a thread: with few rows one as long as 512 threads cover a row, for a row's time is then its chain of loads,
+// sums and stores, and more warps bring it in sooner; with many rows four, so that more rows are under way on an SM and what a warp does
+// once for a row serves more of it (4096 rows of 4096, bfloat16 in, e4m3 out: 64 us with one piece, GN_MANY with four).
 template <bool VEC>
-static int gn_launch(const GnParams& p, int T, cudaStream_t stream) {
+static int gn_launch(const GnParams& p, int T, int sms, cudaStream_t stream) {
     const int pieces = (p.H + 7) / 8;
     auto threads = [&](int c) { return ((pieces + c - 1) / c + 31) / 32 * 32; };
-    if (threads(1) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 1>, T, threads(1), 0, stream, p);
-    else if (threads(2) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 2>, T, threads(2), 0, stream, p);
+    const bool few = T <= 2 * sms;
+    if (few && threads(1) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 1>, T, threads(1), 0, stream, p);
+    else if (few && threads(2) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 2>, T, threads(2), 0, stream, p);
     else if (threads(4) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 4>, T, threads(4), 0, stream, p);
     else return ACV_ERR_SIZE;
     return acv_launch_status();
@@ -170,8 +182,8 @@ static int gn_launch(const GnParams& p, int T, cudaStream_t stream) {
 struct GatedNormsArgs {
     const void *x, *d, *g, *gc, *w1, *w2, *out, *s, *stream;
     long long ldx, ldd, ldg, ldo, lds;
-    int x_dtype, d_dtype, g_dtype, out_kind, T, H;
-    float c, e1, e2;
+    int x_dtype, d_dtype, g_dtype, out_kind, T, H, sms;
+    float c, e1, e2, inv_h;
 };
 ACV_API int acv_add_gated_norms(const GatedNormsArgs* a) {
     const int T = a->T, H = a->H;
@@ -184,12 +196,12 @@ ACV_API int acv_add_gated_norms(const GatedNormsArgs* a) {
     p.out = const_cast<void*>(a->out); p.s = (float*)const_cast<void*>(a->s);
     p.ldx = a->ldx; p.ldd = a->ldd; p.ldg = a->ldg; p.ldo = a->ldo; p.lds = a->lds; p.H = H;
     p.x_f32 = a->x_dtype == ACV_F32; p.d_f32 = a->d_dtype == ACV_F32; p.g_f32 = a->g_dtype == ACV_F32; p.out_kind = a->out_kind;
-    p.c = a->c; p.e1 = a->e1; p.e2 = a->e2;
+    p.c = a->c; p.e1 = a->e1; p.e2 = a->e2; p.inv_h = 1.f / (float)H;
     const int ob = p.out_kind == 0 ? 4 : p.out_kind == 1 ? 2 : 1;
     const bool vec = H % 8 == 0 && fp8_rows_aligned(p.x, p.ldx, p.x_f32 ? 4 : 2, 16) && (!p.d || fp8_rows_aligned(p.d, p.ldd, p.d_f32 ? 4 : 2, 16)) &&
                      (!p.g || fp8_rows_aligned(p.g, p.ldg, p.g_f32 ? 4 : 2, 16)) &&
                      (p.out_kind == 3 || fp8_rows_aligned(p.out, p.ldo, ob, p.out_kind == 2 ? 8 : 16)) &&
                      !(((uintptr_t)p.gc | (uintptr_t)p.w1 | (uintptr_t)p.w2) & 15);
     const cudaStream_t stream = (cudaStream_t)const_cast<void*>(a->stream);
-    return vec ? gn_launch<true>(p, T, stream) : gn_launch<false>(p, T, stream);
+    return vec ? gn_launch<true>(p, T, a->sms, stream) : gn_launch<false>(p, T, a->sms, stream);
 }

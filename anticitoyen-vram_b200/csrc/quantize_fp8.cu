@@ -4,11 +4,12 @@
 
 // Rows: sixteen lanes hold a group, eight neighbouring elements each, so the group's maximum takes four exchanges and no shared
 // memory.  A half-warp takes U groups at once, their loads in flight together, and goes on by the grid's stride; the stride in
-// (rows, groups) comes from the host, so no group costs a division.
+// (rows, groups) comes from the host, so no group costs a division for its place.  The scales' two divisions cost more than the rest of
+// a group together: a half-warp's lanes make those of its U groups side by side, once.
 template <bool VEC, int U>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int f32, long long ldx, uint8_t* __restrict__ q,
-                                                            long long ldq, float* __restrict__ s, long long lds, int T, int K, int G,
-                                                            int step_rows, int step_groups) {
+__global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const void* __restrict__ x, int f32, long long ldx, uint8_t* __restrict__ q,
+                                                               long long ldq, float* __restrict__ s, long long lds, int T, int K, int G,
+                                                               int step_rows, int step_groups) {
     pdl_launch_dependents();
     pdl_wait();
     const int lane = threadIdx.x & 15;
@@ -19,7 +20,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
     while (__any_sync(0xffffffffu, row < T)) {
         int rows[U], gs[U];
         Raw8 raw[U];
-        float v[U][8];
+        float v[8];
+        uint32_t own = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             rows[u] = row;
@@ -28,23 +30,29 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
             g += step_groups;
             if (g >= G) { g -= G; ++row; }
             const int at = gs[u] * FP8_GROUP + lane * 8;
-            const bool in = rows[u] < T && at < K;
             const char* src = reinterpret_cast<const char*>(x) + (size_t)rows[u] * ldx * esz;
-            if (VEC) {
-                raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
-                if (in) raw[u] = raw8_load(src, f32, at);
-            } else {
-                load8_ragged(src, f32, at, in ? K : 0, v[u]);
+            raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
+            if (rows[u] < T && at < K) {
+                if (VEC) raw[u] = raw8_load(src, f32, at);
+                else raw[u] = raw8_load_ragged(src, f32, at, K);
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (VEC) raw8_floats(raw[u], f32, v[u]);
-            const Fp8Scale k = fp8_scale(half_warp_max(magnitude8(v[u])));
+            const uint32_t m = half_warp_max(magnitude8(raw[u], f32));
+            if (lane % U == u) own = m;
+        }
+        const Fp8Scale mine = fp8_scale(own);           // of group lane % U
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float r = __shfl_sync(0xffffffffu, mine.r, u, 16);
             const int at = gs[u] * FP8_GROUP + lane * 8;
             if (rows[u] < T) {
-                if (at < K) store_q8<VEC>(q + (size_t)rows[u] * ldq, at, K, v[u], k.r);
-                if (lane == 0) s[(size_t)rows[u] * lds + gs[u]] = k.s;
+                if (at < K) {
+                    raw8_floats(raw[u], f32, v);
+                    store_q8<VEC>(q + (size_t)rows[u] * ldq, at, K, v, r);
+                }
+                if (lane == u) s[(size_t)rows[u] * lds + gs[u]] = mine.s;
             }
         }
     }
@@ -64,20 +72,16 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __rest
     Raw8 raw[8];
     float v[8];
     uint32_t m = 0;
-    if (VEC) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            raw[i].a = raw[i].b = make_uint4(0, 0, 0, 0);
-            if (row0 + 16 * i < T && at < K)
-                raw[i] = raw8_load(reinterpret_cast<const char*>(x) + (size_t)(row0 + 16 * i) * ldx * esz, f32, at);
+    for (int i = 0; i < 8; ++i) {
+        raw[i].a = raw[i].b = make_uint4(0, 0, 0, 0);
+        if (row0 + 16 * i < T && at < K) {
+            const char* src = reinterpret_cast<const char*>(x) + (size_t)(row0 + 16 * i) * ldx * esz;
+            raw[i] = VEC ? raw8_load(src, f32, at) : raw8_load_ragged(src, f32, at, K);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (VEC) raw8_floats(raw[i], f32, v);
-        else load8_ragged(reinterpret_cast<const char*>(x) + (size_t)(row0 + 16 * i) * ldx * esz, f32, at, row0 + 16 * i < T ? K : 0, v);
-        m = max(m, magnitude8(v));
-    }
+    for (int i = 0; i < 8; ++i) m = max(m, magnitude8(raw[i], f32));
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
     __syncthreads();
@@ -89,8 +93,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __rest
     for (int i = 0; i < 8; ++i) {
         const int row = row0 + 16 * i;
         if (row >= T || at >= K) continue;
-        if (VEC) raw8_floats(raw[i], f32, v);
-        else load8_ragged(reinterpret_cast<const char*>(x) + (size_t)row * ldx * esz, f32, at, K, v);
+        raw8_floats(raw[i], f32, v);
         store_q8<VEC>(q + (size_t)row * ldq, at, K, v, k.r);
     }
 }
@@ -125,12 +128,12 @@ ACV_API int acv_quantize_fp8(const QuantizeFp8Args* a) {
     if (block_rows != 1) return ACV_ERR_SIZE;
     const long long groups = (long long)T * G;
     const long long blocks = (groups + 15) / 16;
-    const int grid = (int)(blocks < (long long)sms * 8 ? blocks : (long long)sms * 8);
+    const int grid = (int)(blocks < (long long)sms * 4 ? blocks : (long long)sms * 4);
     const long long stride = (long long)grid * 16;
     const int step_rows = (int)(stride / G), step_groups = (int)(stride % G);
     if ((long long)T + 4ll * (step_rows + 1) > 0x7fffffffll) return ACV_ERR_SIZE;
     if (!vec)
-        acv_launch(PDL_MISC, quantize_rows_kernel<false, 1>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K, G, step_rows, step_groups);
+        acv_launch(PDL_MISC, quantize_rows_kernel<false, 2>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K, G, step_rows, step_groups);
     else
         acv_launch(PDL_MISC, quantize_rows_kernel<true, 4>, grid, 256, 0, stream, x, f32, ldx, q, ldq, s, lds, T, K, G, step_rows, step_groups);
     return acv_launch_status();

@@ -2395,7 +2395,7 @@ def fp8_rows(rows: int, columns: int, device) -> tuple[torch.Tensor, torch.Tenso
 # and only a call that is refused, or has a column of a single element, goes through the words about it.
 _LINEAR_ARGS = struct.Struct("@10Q8q7i")        # Fp8LinearArgs
 _QUANTIZE_ARGS = struct.Struct("@4Q3q5i")       # QuantizeFp8Args
-_NORMS_ARGS = struct.Struct("@9Q5q6i3f")        # GatedNormsArgs
+_NORMS_ARGS = struct.Struct("@9Q5q7i3f")        # GatedNormsArgs
 _entries: dict = {}
 
 
@@ -2593,5 +2593,5 @@ def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tens
         _one_device(name, x, delta, gate, post_weight, weight if out is not None else None, out, out_scales)
     if T and H:
         _launch_record(device, name, _NORMS_ARGS, 8, x.data_ptr(), d_at, g_at, gc_at, w1_at, w2_at, out_at, s_at, xs[0], d_ld, g_ld, out_ld,
-                       s_ld, _DT[x.dtype], d_type, g_type, kind, T, H, residual_scale, post_eps, eps)
+                       s_ld, _DT[x.dtype], d_type, g_type, kind, T, H, _sms_of(device), residual_scale, post_eps, eps)
     return out
