@@ -278,15 +278,15 @@ def time_parts(runner, q_lens: list, kv_lens: list, reps: int = 5, layer: int = 
 
 
 def bench_decode(model, random_weights=False, seed=0, dtype="bfloat16", batches=(1,), context=128, n_tokens=256,
-                 device="cuda:0", cuda_graphs=True, repetitions=3, prefill=0) -> dict:
+                 device="cuda:0", cuda_graphs=True, repetitions=3, prefill=0, weights=None) -> dict:
     """``acvram bench --what decode``: median decode tokens/s for each batch size, with the spread; with
     ``prefill`` > 0 also the tokens/s of one prompt of that many tokens computed in one step."""
     from .engine import Engine
     need = max(max(batches) * (context + n_tokens + 64), prefill + 64)
     eng = Engine(model, dtype, max_batch_size=max(batches), max_model_len=max(context + n_tokens, prefill) + 64,
                  random_weights=random_weights, seed=seed, device=device, enable_cuda_graphs=cuda_graphs,
-                 page_size=64, num_pages=need // 64 + 2 * max(batches), enable_prefix_cache=False)
-    out = {"model": str(model), "dtype": dtype, "context": context, "tokens": n_tokens}
+                 page_size=64, num_pages=need // 64 + 2 * max(batches), enable_prefix_cache=False, weights=weights)
+    out = {"model": str(model), "dtype": dtype, **({"weights": weights} if weights else {}), "context": context, "tokens": n_tokens}
     for b in batches:
         rates = []
         for rep in range(repetitions):

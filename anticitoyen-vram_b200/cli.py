@@ -26,6 +26,8 @@ def _engine_args(p: argparse.ArgumentParser, model_optional: bool = False) -> No
     p.add_argument("--random-weights", action="store_true", help="ignore the folder's weights; draw them from --seed")
     p.add_argument("--seed", type=int, default=0, help="seed of random weights and of sampling")
     p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    p.add_argument("--weights", default=None, choices=["fp8"],
+                   help="the layers' matrices in 8 bits with block scales, whatever the folder holds (default: as its configuration says)")
     p.add_argument("--max-model-len", type=int, default=8192)
     p.add_argument("--max-batch", type=int, default=16)
     p.add_argument("--page-size", type=int, default=64)
@@ -42,7 +44,7 @@ def _make_engine(args):
     return Engine(args.model, args.dtype, max_batch_size=args.max_batch, max_model_len=args.max_model_len,
                   page_size=args.page_size, num_pages=args.num_pages, token_budget=args.token_budget,
                   random_weights=args.random_weights, seed=args.seed, device=args.device,
-                  enable_cuda_graphs=not args.no_cuda_graphs, enable_prefix_cache=not args.no_prefix_cache)
+                  enable_cuda_graphs=not args.no_cuda_graphs, enable_prefix_cache=not args.no_prefix_cache, weights=args.weights)
 
 
 def cmd_generate(args) -> int:
@@ -94,7 +96,7 @@ def cmd_bench(args) -> int:
     res = bench_decode(args.model, random_weights=args.random_weights, seed=args.seed, dtype=args.dtype,
                        batches=[int(b) for b in args.batch.split(",")], context=args.context,
                        n_tokens=args.tokens, device=args.device, cuda_graphs=not args.no_cuda_graphs,
-                       prefill=args.prefill)
+                       prefill=args.prefill, weights=args.weights)
     if args.json:
         print(json.dumps(res))
     else:

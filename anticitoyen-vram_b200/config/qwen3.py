@@ -33,6 +33,8 @@ class Qwen3Config:
     hidden_act: str = "silu"
     eos_token_id: tuple[int, ...] = ()
     bos_token_id: int | None = None
+    # the layers' matrices in e4m3 with a scale for each block of 128 x 128 ("quantization_config" of quant_method "fp8")
+    weights_fp8: bool = False
 
     architecture = "Qwen3ForCausalLM"
     model_type = "qwen3"
@@ -69,10 +71,24 @@ class Qwen3Config:
             hidden_act=str(act),
             eos_token_id=take_id_list(cfg, "eos_token_id"),
             bos_token_id=bos if isinstance(bos, int) and not isinstance(bos, bool) else None,
+            weights_fp8=cls._weights_fp8(cfg),
         )
         self._check_unsupported(cfg)
         self.validate()
         return self
+
+    @staticmethod
+    def _weights_fp8(cfg: Mapping[str, Any]) -> bool:
+        """Whether the configuration asks for 8-bit weights; what is built of them is the form with block scales and activations
+        quantised as they come.  (Other methods are no business of this key's reader: their files hold other tensors.)"""
+        quant = cfg.get("quantization_config")
+        if not isinstance(quant, Mapping) or quant.get("quant_method") != "fp8":
+            return False
+        for key, want, default in (("weight_block_size", [128, 128], None), ("activation_scheme", "dynamic", "dynamic"), ("fmt", "e4m3", "e4m3")):
+            got = quant.get(key, default)
+            if (list(got) if isinstance(got, (list, tuple)) else got) != want:
+                raise ConfigError(f"config key 'quantization_config': '{key}' is {got!r}; of 8-bit weights {want!r} is built")
+        return True
 
     @staticmethod
     def _check_unsupported(cfg: Mapping[str, Any]) -> None:
@@ -118,4 +134,6 @@ class Qwen3Config:
         out["eos_token_id"] = eos[0] if len(eos) == 1 else (eos or None)
         out["architectures"] = [self.architecture]
         out["model_type"] = self.model_type
+        if out.pop("weights_fp8"):
+            out["quantization_config"] = {"quant_method": "fp8", "fmt": "e4m3", "activation_scheme": "dynamic", "weight_block_size": [128, 128]}
         return out

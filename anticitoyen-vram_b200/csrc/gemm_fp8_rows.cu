@@ -121,12 +121,12 @@ __global__ void __launch_bounds__(RR_WARPS * 32, 2) gemm_fp8_rows_kernel(const F
 #pragma unroll
             for (int i = 0; i < 4; ++i) total[a][h][i] = 0.f;
     const float* sw = p.sw + (size_t)(n0 / FP8_GROUP) * p.ldsw + c0;
-    float scale = chunks ? __ldg(sw) : 0.f;
+    float scale = chunks ? sw[0] : 0.f;
     int from = 0;
 #pragma unroll 1
     for (int n = 0; n < chunks; ++n) {
         const float s = scale;
-        if (n + 1 < chunks) scale = __ldg(sw + n + 1);
+        if (n + 1 < chunks) scale = sw[n + 1];
         cp_async_wait<DEPTH - 2>();
         Chunk chunk;
         chunk.read(own + from * CHUNK);

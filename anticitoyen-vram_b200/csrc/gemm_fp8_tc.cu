@@ -48,11 +48,11 @@ struct FtRowScales {
     float now[4], next[4];
     __device__ __forceinline__ void fetch(float (&v)[4]) {
         if (vec && left >= 4) {
-            const float4 f = __ldg(reinterpret_cast<const float4*>(at));
+            const float4 f = *reinterpret_cast<const float4*>(at);
             v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = i < left ? __ldg(at + i) : 0.f;
+            for (int i = 0; i < 4; ++i) v[i] = i < left ? at[i] : 0.f;
         }
         at += 4;
         left -= 4;
@@ -252,12 +252,12 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             for (int i = 0; i < 64; ++i) sums[i] = 0;
             FtRowScales xs;
             xs.begin(sx, p.n_kb, p.sx_vec);
-            float next_w = __ldg(sw), next_w2 = GATED ? __ldg(sw2) : 0.f;
+            float next_w = sw[0], next_w2 = GATED ? sw2[0] : 0.f;
             for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
                 const float x = xs.take(kb), s1 = x * next_w, s2 = GATED ? x * next_w2 : s1;
                 if (kb + 1 < p.n_kb) {
-                    next_w = __ldg(sw + kb + 1);
-                    if (GATED) next_w2 = __ldg(sw2 + kb + 1);
+                    next_w = sw[kb + 1];
+                    if (GATED) next_w2 = sw2[kb + 1];
                 }
                 const uint32_t slot = turn % FP_SLOTS, use = turn / FP_SLOTS;
                 failed = ft_warp_failed(tfull0 + 8 * slot, use & 1, &abort_s, p);
@@ -443,13 +443,13 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         for (int i = 0; i < S::COLS / 2; ++i) sums[i] = 0;
         FtRowScales xs;
         xs.begin(sx + kb0, kb1 - kb0, p.sx_vec && !(kb0 & 3));
-        float next_w = __ldg(sw + kb0), next_w2 = GATED ? __ldg(sw2 + kb0) : 0.f;
+        float next_w = sw[kb0], next_w2 = GATED ? sw2[kb0] : 0.f;
         uint32_t turn = 0;
         for (int kb = kb0; kb < kb1; ++kb, ++turn) {
             const float a = xs.take((int)turn), b = next_w, b2 = next_w2;
             if (kb + 1 < kb1) {
-                next_w = __ldg(sw + kb + 1);
-                if (GATED) next_w2 = __ldg(sw2 + kb + 1);
+                next_w = sw[kb + 1];
+                if (GATED) next_w2 = sw2[kb + 1];
             }
             const uint32_t buf = turn % S::SLOTS, use = turn / S::SLOTS;
             if (ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p)) break;

@@ -90,7 +90,7 @@ class Engine:
                  page_size: int = 64, num_pages: int | None = None, token_budget: int = 2048,
                  random_weights: bool = False, seed: int = 0, device: str = "cuda:0",
                  enable_cuda_graphs: bool = True, run_ahead: bool = True, enable_prefix_cache: bool = True,
-                 tokenizer=None, fuse_decode_layers: bool = False) -> None:
+                 tokenizer=None, fuse_decode_layers: bool = False, weights: str | None = None) -> None:
         """``model``: a folder with config.json and model.safetensors, or (with
         ``random_weights``) a typed configuration or a folder whose config.json alone is read.
         ``tokenizer``: anything with ``decode(ids) -> str``; with one, outputs carry the text that their tokens
@@ -98,9 +98,11 @@ class Engine:
         ``enable_prefix_cache`` (the reference's name and default, acvram/engine/runner.py:689-694): the full
         pages of a finished request stay known, and a later request that begins the same way takes them over.
         ``fuse_decode_layers``: steps of up to 16 decoding requests run each layer as one persistent kernel instead
-        of seven launches (slower on a B200 at the sizes measured; kept as a choice)."""
+        of seven launches (slower on a B200 at the sizes measured; kept as a choice).
+        ``weights``: None, as the model's configuration says; "fp8" (Qwen3): the layers' matrices in e4m3 with a scale for
+        each block of 128 x 128, quantised as they are loaded where the folder holds them in more bits."""
         from ..config import load_config
-        from ..models import build_from_folder, build_random
+        from ..models import build_from_folder, build_random, with_weights
 
         run_dtype = _DTYPES[dtype]
         if not torch.cuda.is_available():
@@ -109,10 +111,10 @@ class Engine:
             self.model, self.config = model, None
         elif random_weights:
             config = load_config(model) if isinstance(model, (str, bytes)) or hasattr(model, "__fspath__") else model
-            self.model = build_random(config, seed, run_dtype, device)
-            self.config = config
+            self.config = with_weights(config, weights)
+            self.model = build_random(self.config, seed, run_dtype, device)
         else:
-            self.config, self.model = build_from_folder(model, run_dtype, device)
+            self.config, self.model = build_from_folder(model, run_dtype, device, weights)
         plan = self.model.plan
         for block in getattr(self.model, "blocks", ()):
             if hasattr(block, "fuse_decode"):

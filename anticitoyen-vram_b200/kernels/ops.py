@@ -2523,6 +2523,7 @@ def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tenso
     return out, out_scales
 
 
+GATED_NORMS_WIDTH = 16384       # elements of a row that a block holds in its registers (csrc/gated_norms.cu)
 _NORM_OUT = {torch.float32: 0, torch.bfloat16: 1, FP8: 2}
 
 

@@ -53,6 +53,7 @@ class CacheView:
 
 class Part:
     kind = "?"
+    takes_fp8 = False     # its input may come as ``Fp8Rows`` (parts/linear.py): its first products are 8-bit ones
     capturable = True     # forward only launches kernels (no read of device memory by the host): may run in a CUDA graph
 
     def tensor_needs(self) -> Mapping[str, TensorNeed]:

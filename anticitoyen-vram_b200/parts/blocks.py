@@ -182,12 +182,18 @@ class PreNormBlock:
             h = self._normed_conv(x, delta, ctx, cache.parts["conv"], kw, scale)
             cache = cache.parts.get("mixer")
         else:
-            h = self.input_norm.forward(x, delta, **kw, **scale)
+            h = self._normed(self.input_norm, x, delta, self.mixer, kw, scale)
         a = self.mixer.forward(h, ctx, cache)
         if self.feed_forward is None:
             return x, a
-        h = self.post_norm.forward(x, a, **kw, **scale)
+        h = self._normed(self.post_norm, x, a, self.feed_forward, kw, scale)
         return x, self.feed_forward.forward(h, ctx)
+
+    def _normed(self, norm, x, delta, part, kw: dict, scale: dict):
+        """The sum and its norm, in 8 bits where the part behind it reads that."""
+        if part.takes_fp8 and getattr(norm, "groups", 0) == 1 and x.shape[1] <= ops.GATED_NORMS_WIDTH:
+            return norm.forward_fp8(x, delta, self.run_dtype, **scale)
+        return norm.forward(x, delta, **kw, **scale)
 
 
 @register("block", "parallel")

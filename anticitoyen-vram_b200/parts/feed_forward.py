@@ -9,7 +9,7 @@ import torch
 from ..kernels import ops
 from ..weights.needs import TensorNeed
 from .base import FeedForward, Runtime
-from .linear import Linear
+from .linear import Fp8Linear, Fp8Rows, Linear
 from .registry import register
 
 
@@ -19,8 +19,9 @@ class SwiGLU(FeedForward):
     (acvram/engine/attention.py:705-783)."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, prefix: str = "mlp.", bias: bool | None = None,
-                 names: dict | None = None, activation: str = "silu", limit: float = 0.0, alpha: float = 0.0) -> None:
-        """``bias``: True, the three projections have biases; False, none; None, those that the file holds.
+                 names: dict | None = None, activation: str = "silu", limit: float = 0.0, alpha: float = 0.0, fp8: bool = False) -> None:
+        """``fp8``: the three matrices in 8 bits with block scales (``Fp8Linear``); the unit's output is quantised as it leaves the first
+        product, for the second.  silu, no biases.  ``bias``: True, the three projections have biases; False, none; None, those that the file holds.
         ``names``: the tensors' names behind ``prefix``, {"gate": w, "gate.bias": b, "up": ..., "down": ...}.
         ``activation``: what the gate passes through, "silu" or "gelu_tanh" (0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3)))),
         computed in float; or "swish_clamped": with g = min(gate, limit) and u = clamp(up, -limit, limit) the unit is
@@ -29,6 +30,9 @@ class SwiGLU(FeedForward):
             raise ValueError(f"gated feed-forward: no activation '{activation}' (silu, gelu_tanh and swish_clamped are built)")
         if activation == "swish_clamped" and not limit > 0.0:
             raise ValueError("gated feed-forward: swish_clamped wants a positive limit")
+        if fp8 and (activation != "silu" or bias):
+            raise ValueError("gated feed-forward: 8-bit weights are built for silu without biases")
+        self.takes_fp8 = self.fp8 = bool(fp8)
         self.activation = activation
         self.limit, self.alpha = float(limit), float(alpha)
         self.inner_size = intermediate_size
@@ -45,18 +49,29 @@ class SwiGLU(FeedForward):
         H, I = self.hidden_size, self.intermediate_size
         needs = {}
         for role, n_out, n_in in (("gate", I, H), ("up", I, H), ("down", H, I)):
+            if self.fp8:
+                needs.update(Fp8Linear.needs(self.prefix + self.names[role], n_out, n_in))
+                continue
             needs[self.prefix + self.names[role]] = TensorNeed((n_out, n_in))
             if self.bias is not False and role + ".bias" in self.names:
                 needs[self.prefix + self.names[role + ".bias"]] = TensorNeed((n_out,), "bias", optional=self.bias is None)
         return needs
 
     def weight_bytes(self) -> int:
+        if self.fp8:
+            return self.gate.weight_bytes() + self.up.weight_bytes() + self.down.weight_bytes()
         return self.gate_up.weight_bytes() + self.down.weight_bytes()
 
     def flops(self, num_tokens: int) -> float:
+        if self.fp8:
+            return self.gate.flops(num_tokens) + self.up.flops(num_tokens) + self.down.flops(num_tokens)
         return self.gate_up.flops(num_tokens) + self.down.flops(num_tokens)
 
     def load(self, tensors, rt: Runtime) -> None:
+        if self.fp8:
+            self.gate, self.up, self.down = (Fp8Linear([Fp8Linear.matrix(tensors, self.prefix + self.names[role], rt.device)])
+                                             for role in ("gate", "up", "down"))
+            return
         w = lambda role: tensors[self.prefix + self.names[role]].to(device=rt.device, dtype=rt.dtype)
 
         def b(role):
@@ -84,12 +99,14 @@ class SwiGLU(FeedForward):
 
     def decode_layer_spec(self):
         """What the fused decode-layer kernel needs of this feed-forward: gate and up rows interleaved, no biases."""
-        if not self.fused or self.down.bias is not None or self.gate_up.bias is not None or self.activation != "silu":
+        if self.fp8 or not self.fused or self.down.bias is not None or self.gate_up.bias is not None or self.activation != "silu":
             return None
         return {"intermediate_size": self.intermediate_size, "w_gate_up_pairs": self.gate_up.weight, "w_down": self.down.weight}
 
     def inner(self, h, ctx, out) -> None:
         """The unit's output in front of the down product into ``out`` [T, inner_size] (dense rows at any stride)."""
+        if self.fp8:
+            raise ValueError("gated feed-forward: 8-bit weights do not share a product with another part's")
         if self.fused and self.fused_act is not None and h.shape[0] and ops.gemm_tc_takes(h, self.gate_up.weight):
             ops.linear_bf16_swiglu(h, self.gate_up.weight, out, static_weights=True, bias=self.gate_up.bias,
                                    **({"act": self.fused_act} if self.activation != "silu" else {}),
@@ -109,6 +126,11 @@ class SwiGLU(FeedForward):
                 ops.glu(gu, out, ops.ACTIVATIONS["silu"], 0.0, 0.0)
 
     def forward(self, h, ctx):
+        if self.fp8:
+            h = Fp8Rows.of(h)
+            act = Fp8Rows(h.shape[0], self.intermediate_size, h.device, h.dtype)
+            ops.linear_fp8_swiglu(h.values, h.scales, *self.gate.matrices[0], *self.up.matrices[0], act.values, act.scales)
+            return self.down(act)
         act = h.new_empty((h.shape[0], self.intermediate_size))
         self.inner(h, ctx, act)
         return self.down(act)

@@ -8,7 +8,7 @@ from ..cache.manager import PagedNeed
 from ..kernels import ops
 from ..weights.needs import TensorNeed
 from .base import CacheView, Mixer, Runtime, StepMetadata
-from .linear import Linear
+from .linear import Fp8Linear, Linear
 from .plan import PartSpec
 from .position import NoPosition
 from .registry import build, register
@@ -52,7 +52,9 @@ class Attention(Mixer):
     of query i and key j, slope_h = 2^(-r (h + 1) / heads).
     ``tied_values``: there is no value projection; a head's value is its key as projected, before norm and rotation (both are
     kept, one beside the other).  ``gate``: the name of a matrix W_g over the heads' values: the heads side by side are
-    multiplied by sigmoid(W_g h) in front of W_o, in the attention kernels, in 32-bit, before they are rounded."""
+    multiplied by sigmoid(W_g h) in front of W_o, in the attention kernels, in 32-bit, before they are rounded.
+    ``fp8``: the projections' matrices in 8 bits with block scales (``Fp8Linear``), no biases; what they give, the cache and the
+    attention are in the run's element type."""
 
     ROLES = ("q", "k", "v", "o")
 
@@ -62,7 +64,10 @@ class Attention(Mixer):
                  names: dict | None = None, out_scale: float = 1.0, qk_norm_weights: bool = True,
                  score: dict | None = None, qk_norm_scope: str = "head", value_norm_eps: float | None = None,
                  q_temp: tuple | None = None, value_share: dict | None = None, sink: str | float | None = None,
-                 slope_rate: float | None = None, tied_values: bool = False, gate: str | None = None) -> None:
+                 slope_rate: float | None = None, tied_values: bool = False, gate: str | None = None, fp8: bool = False) -> None:
+        if fp8 and (tied_values or gate is not None or bias):
+            raise ValueError("attention: 8-bit weights are not built beside tied values, an output gate or biases")
+        self.takes_fp8 = self.fp8 = bool(fp8)
         if num_heads % num_kv_heads:
             raise ValueError(f"{num_heads} heads are not a multiple of {num_kv_heads} kv heads")
         if qk_norm_scope not in ("head", "all"):
@@ -144,6 +149,9 @@ class Attention(Mixer):
                                   ("o", H, self.inner_size)):
             if role == "v" and self.tied_values:
                 continue
+            if self.fp8:
+                needs.update(Fp8Linear.needs(self.prefix + self.names[role], n_out, n_in))
+                continue
             needs[self.prefix + self.names[role]] = TensorNeed((n_out, n_in))
             if self.bias is not False and role + ".bias" in self.names:
                 needs[self.prefix + self.names[role + ".bias"]] = TensorNeed((n_out,), "bias", optional=self.bias is None)
@@ -174,13 +182,17 @@ class Attention(Mixer):
             name = self.prefix + self.names.get(role + ".bias", "\0")
             return tensors[name].to(device=rt.device, dtype=torch.float32) if name in tensors else None
 
-        roles = ("q", "k") if self.tied_values else ("q", "k", "v")
-        rows, biases = [w(r) for r in roles], [b(r) for r in roles]
-        if self.gate is not None:
-            rows.append(tensors[self.prefix + self.gate].to(device=rt.device, dtype=rt.dtype))
-            biases.append(None)
-        self.qkv = Linear.stacked(rows, biases)
-        self.o = Linear(w("o"), b("o"))
+        if self.fp8:
+            q, k, v, o = (Fp8Linear.matrix(tensors, self.prefix + self.names[r], rt.device) for r in self.ROLES)
+            self.qkv, self.o = Fp8Linear([q, k, v]), Fp8Linear([o])
+        else:
+            roles = ("q", "k") if self.tied_values else ("q", "k", "v")
+            rows, biases = [w(r) for r in roles], [b(r) for r in roles]
+            if self.gate is not None:
+                rows.append(tensors[self.prefix + self.gate].to(device=rt.device, dtype=rt.dtype))
+                biases.append(None)
+            self.qkv = Linear.stacked(rows, biases)
+            self.o = Linear(w("o"), b("o"))
         self.q_norm = self.k_norm = None
         f = lambda n: tensors[n].to(device=rt.device, dtype=torch.float32).contiguous()
         if self.qk_norm_eps is not None and self.qk_norm_weights:
@@ -214,7 +226,7 @@ class Attention(Mixer):
         """What the fused decode-layer kernel needs of this mixer (it knows rotary positions over the whole head,
         applied by table, and no biases)."""
         rotary = self.position.rotary_table()
-        if self.qkv.bias is not None or self.o.bias is not None or rotary is None or rotary.shape[1] != self.head_dim \
+        if self.fp8 or self.qkv.bias is not None or self.o.bias is not None or rotary is None or rotary.shape[1] != self.head_dim \
                 or self.value_dim != self.head_dim or self.keep_first or self.out_scale != 1.0 or self.wide \
                 or self.sinks is not None or self.slopes is not None or self.score is not None or self.tied_values \
                 or self.gate is not None:
@@ -337,7 +349,7 @@ class Attention(Mixer):
         kp, vp = (cache.k_pages, cache.v_pages) if cache.writes else (None, None)
         eps = self.qk_norm_eps if self.qk_norm_eps is not None else 0.0
         rotary = self.position.rotary_table()
-        if rotary is not None and self.qkv.bias is None and ops.gemm_tc_qkv_takes(h, self.qkv.weight, D, rotary, kp):
+        if rotary is not None and not self.fp8 and self.qkv.bias is None and ops.gemm_tc_qkv_takes(h, self.qkv.weight, D, rotary, kp):
             # a few tokens: norm, rotation and append ride on the projection's kernel as its tile leaves
             qkv = h.new_empty((h.shape[0], self.qkv.out_features))
             ops.gemm_tc_qkv(h, self.qkv.weight, qkv, NH, NKV, D, self.q_norm, self.k_norm, eps, rotary, ctx.positions,

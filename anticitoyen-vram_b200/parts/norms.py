@@ -7,6 +7,7 @@ import torch
 from ..kernels import ops
 from ..weights.needs import TensorNeed
 from .base import Norm, Runtime
+from .linear import Fp8Rows
 from .registry import register
 
 
@@ -61,6 +62,14 @@ class RMSNorm(Norm):
         if x.dtype == torch.float32 and out_dtype != torch.float32:
             return ops.add_rmsnorm_f32(x, delta, self.weight, self.eps, out, rows)
         return ops.add_rmsnorm(x, delta, self.weight, self.eps, out, rows)
+
+
+    def forward_fp8(self, x, delta, dtype: torch.dtype, delta_scale: float = 1.0) -> Fp8Rows:
+        """The same for a part whose first products are 8-bit ones: sum, norm and quantisation in one kernel; ``dtype``: the
+        parts' element type.  The norm's output is not rounded in between."""
+        rows = Fp8Rows(x.shape[0], x.shape[1], x.device, dtype)
+        ops.add_gated_norms(x, delta, rows.values, rows.scales, residual_scale=delta_scale, weight=self.weight, eps=self.eps)
+        return rows
 
 
 @register("norm", "layernorm")

@@ -13,7 +13,7 @@ and skipped, unless ``strict`` asks for the error; beside another fault they are
 listed in the error with it.
 
 Storage rule: bfloat16 stays bfloat16, float32 stays float32, integer tables
-become int32.  float16 becomes float32, which holds every float16 value exactly
+become int32; e4m3 is kept where a part asks for it (role "fp8").  float16 becomes float32, which holds every float16 value exactly
 (bfloat16 would drop three bits of its mantissa): a float32 run then computes
 with the file's own values, and a bfloat16 run rounds them once, where the parts
 cast what they compute with.
@@ -90,6 +90,8 @@ def load_tensors(folder: str | os.PathLike, needs: Mapping[str, TensorNeed],
                 continue
             tensor = handles[present[name][0]].get_tensor(name)
             keep = _KEEP.get(tensor.dtype)
+            if needs[name].role == "fp8" and tensor.dtype == torch.float8_e4m3fn:
+                keep = tensor.dtype
             if keep is None:
                 wrong_dtype.append((name, str(tensor.dtype)))
                 continue

@@ -10,7 +10,8 @@ class TensorNeed:
     """One tensor that a part reads by name.
 
     ``role`` decides the random initialisation ("matrix", "embedding" and "bias":
-    N(0, 0.02); "norm": 1 + N(0, 0.1); "table": integers) and nothing else;
+    N(0, 0.02); "norm": 1 + N(0, 0.1); "table": integers) and, for "fp8", the storage:
+    a matrix that the file may hold in e4m3, which is then kept as it is;
     ``optional`` tensors may be absent from the file (a tied output head).
     A dimension written -1 is the file's to choose (a table whose number of rows no
     configuration key names: the part reads it from the tensor it is given); a

@@ -98,3 +98,78 @@ def test_plain_quantisation_is_near_what_it_stands_for():
         q, s = pf.quantize(x, block_rows)
         off = (pf.values(q, s, block_rows) - x.double()).abs()
         assert bool((off <= x.double().abs() * 2.0 ** -4 * (1 + 1e-6) + pf.spread(s.double(), 200, 300, block_rows) * 2.0 ** -10).all())
+
+
+# ----------------------------------------------------------------------------- configurations and weight files
+def fp8_config(**quant):
+    from conftest import tiny_config
+    cfg = tiny_config("F").to_dict()
+    cfg["quantization_config"] = {"quant_method": "fp8", "fmt": "e4m3", "activation_scheme": "dynamic", "weight_block_size": [128, 128], **quant}
+    return cfg
+
+
+def test_configuration_of_8_bit_weights():
+    from acvram_b200.config import ConfigError, Qwen3Config
+    from conftest import tiny_config
+    cfg = Qwen3Config.from_dict(fp8_config())
+    assert cfg.weights_fp8 and Qwen3Config.from_dict(cfg.to_dict()) == cfg
+    assert "quantization_config" not in tiny_config("F").to_dict() and "weights_fp8" not in tiny_config("F").to_dict()
+    assert not Qwen3Config.from_dict(fp8_config(quant_method="other")).weights_fp8
+    for patch in ({"weight_block_size": [64, 128]}, {"weight_block_size": None}, {"activation_scheme": "static"}, {"fmt": "e5m2"}):
+        with pytest.raises(ConfigError, match="quantization_config"):
+            Qwen3Config.from_dict(fp8_config(**patch))
+
+
+def test_weights_in_8_bits_are_asked_of_the_configuration():
+    from acvram_b200.config import ConfigError
+    from acvram_b200.models import needs_of_plan, with_weights
+    from acvram_b200.config import family_of
+    from conftest import tiny_config
+    cfg = with_weights(tiny_config("F"), "fp8")
+    needs = needs_of_plan(family_of(cfg.to_dict()).build_plan(cfg))
+    assert needs["model.layers.0.mlp.down_proj.weight"].role == "fp8"
+    scale = needs["model.layers.1.self_attn.q_proj.weight_scale_inv"]
+    assert scale.shape == (4, 2) and scale.optional
+    assert needs["model.embed_tokens.weight"].role == "embedding" and "lm_head.weight_scale_inv" not in needs
+    assert with_weights(cfg, None) is cfg
+    with pytest.raises(ConfigError, match="built"):
+        with_weights(cfg, "int4")
+    with pytest.raises(ConfigError, match="not built for"):
+        with_weights(type("C", (), {"architecture": "Other"})(), "fp8")
+
+
+def test_a_weight_file_with_half_of_a_quantised_matrix():
+    from acvram_b200.parts.linear import Fp8Linear
+    from acvram_b200.weights.needs import WeightError
+    q = torch.zeros((128, 128)).to(FP8)
+    with pytest.raises(WeightError, match="w_scale_inv"):
+        Fp8Linear.matrix({"w": q}, "w", "cpu")
+    with pytest.raises(WeightError, match="beside block scales"):
+        Fp8Linear.matrix({"w": q.float(), "w_scale_inv": torch.ones((1, 1))}, "w", "cpu")
+
+
+def test_loader_keeps_e4m3_where_it_is_asked_for(tmp_path):
+    from safetensors.torch import save_file
+    from acvram_b200.weights import load_tensors
+    from acvram_b200.weights.needs import TensorNeed, WeightError
+    save_file({"w": torch.ones((4, 8)).to(FP8)}, str(tmp_path / "model.safetensors"))
+    assert load_tensors(tmp_path, {"w": TensorNeed((4, 8), "fp8")})["w"].dtype == FP8
+    with pytest.raises(WeightError, match="unsupported dtype"):
+        load_tensors(tmp_path, {"w": TensorNeed((4, 8))})
+
+
+def test_parts_refuse_what_is_not_built_beside_8_bit_weights():
+    from acvram_b200.parts.feed_forward import SwiGLU
+    from acvram_b200.parts.mixers import Attention
+    from acvram_b200.parts.plan import PartSpec
+    with pytest.raises(ValueError, match="8-bit"):
+        SwiGLU(64, 128, activation="gelu_tanh", fp8=True)
+    with pytest.raises(ValueError, match="8-bit"):
+        Attention(64, 4, 2, 16, PartSpec("none", {}), bias=True, fp8=True)
+
+
+def test_command_line_has_the_choice():
+    from acvram_b200.cli import build_parser
+    args = build_parser().parse_args(["generate", "folder", "--weights", "fp8"])
+    assert args.weights == "fp8"
+    assert build_parser().parse_args(["bench", "folder"]).weights is None
