@@ -49,6 +49,14 @@ __device__ __forceinline__ void ft_wait_ld(uint32_t (&r)[16]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
                    "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
+__device__ __forceinline__ void ft_wait_ld2(uint32_t (&r)[32], uint32_t (&q)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]),
+                          "+r"(q[i]), "+r"(q[i + 1]), "+r"(q[i + 2]), "+r"(q[i + 3]), "+r"(q[i + 4]), "+r"(q[i + 5]), "+r"(q[i + 6]), "+r"(q[i + 7])
+                     ::"memory");
+}
 __device__ __forceinline__ void ft_fma2(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t scale) {
     asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(scale));
 }
@@ -78,6 +86,13 @@ __device__ __forceinline__ void ft_drain(uint32_t full0, int stages, int asked, 
     }
 }
 
+// whether a phase is over, asked without waiting: the answer is a shared-memory access away, so it is asked for a turn ahead of its use
+__device__ __forceinline__ bool ft_ready(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok != 0;
+}
 // a wait by a whole warp: true for all of its lanes where it ran out for one
 __device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, volatile int* abort_flag, const Fp8TcParams& p, int code = 4) {
     const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.wait_limit));

@@ -63,42 +63,51 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     pdl_launch_dependents();
 
     if (warp == 0) {
-        if (lane == 0) {
-            auto load_w = [&](int s, int kb) {
-                tma_load_2d(tiles_addr + s * S::STAGE, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS + half * 64);
-                if (GATED) tma_load_2d(tiles_addr + s * S::STAGE + FT_TILE / 2, &map_w2, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS + half * 64);
-            };
-            const int early = p.early_w ? min(STAGES, count) : 0;
+        auto load_w = [&](int s, int kb) {
+            tma_load_2d(tiles_addr + s * S::STAGE, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS + half * 64);
+            if (GATED) tma_load_2d(tiles_addr + s * S::STAGE + FT_TILE / 2, &map_w2, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS + half * 64);
+        };
+        const int early = p.early_w ? min(STAGES, count) : 0;
+        if (ft_elect()) {
             for (int i = 0; i < early; ++i) {
                 mbar_expect_tx(full0 + 8 * i, S::STAGE);
                 load_w(i, kb0 + block_of(i));
             }
-            pdl_wait();
-            int s = 0, asked = 0;
-            uint32_t ph = 0;
-            for (int i = 0; i < count; ++i, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                const bool half_done = i < early;
-                const int kb = kb0 + block_of(i);
-                if (!half_done) {
-                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 1); break; }
-                    mbar_expect_tx(full0 + 8 * s, S::STAGE);
-                }
-                ++asked;
-                if (kb == p.skip_kb) continue;
-                tma_load_2d(tiles_addr + s * S::STAGE + FT_TILE, &map_x, full0 + 8 * s, kb * FT_ROWS, t0);
-                if (!half_done) load_w(s, kb);
-            }
-            if (abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
         }
+        __syncwarp();
+        pdl_wait();
+        int s = 0, asked = 0;
+        uint32_t ph = 0;
+        bool failed = false, ready = false;
+        for (; asked < count; ++asked) {
+            const bool half_done = asked < early;
+            const int kb = kb0 + block_of(asked);
+            if (!half_done && !ready) {
+                failed = ft_warp_failed(empty0 + 8 * s, ph ^ 1, &abort_s, p, 1);
+                if (failed) break;
+            }
+            if (ft_elect()) {
+                if (!half_done) mbar_expect_tx(full0 + 8 * s, S::STAGE);
+                if (kb != p.skip_kb) {
+                    tma_load_2d(tiles_addr + s * S::STAGE + FT_TILE, &map_x, full0 + 8 * s, kb * FT_ROWS, t0);
+                    if (!half_done) load_w(s, kb);
+                }
+            }
+            __syncwarp();
+            if (++s == STAGES) { s = 0; ph ^= 1; }
+            ready = __all_sync(0xffffffffu, ft_ready(empty0 + 8 * s, ph ^ 1));
+        }
+        if (failed || abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
     } else if (warp == 1) {
         pdl_wait();
         const uint32_t idesc = ft_idesc(BT, FT_ROWS);
         const uint64_t a0 = umma_desc(tiles_addr), b0 = umma_desc(tiles_addr + FT_TILE);
-        uint32_t turn = 0, ph = 0;
+        uint32_t ph = 0;
         int s = 0;
-        for (int i = 0; i < count; ++i, ++turn) {
-            const uint32_t slot = turn % S::SLOTS, use = turn / S::SLOTS;
-            if (ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3) ||
+        bool ready = false;
+        for (int i = 0; i < count; ++i) {
+            const uint32_t slot = (uint32_t)i % S::SLOTS, use = (uint32_t)i / S::SLOTS;
+            if ((!ready && ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) ||
                 (use && ft_warp_failed(tempty0 + 8 * slot, (use & 1) ^ 1, &abort_s, p, 2)))
                 break;
             tc_fence_after();
@@ -111,6 +120,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             }
             __syncwarp();
             if (++s == STAGES) { s = 0; ph ^= 1; }
+            ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));
         }
     } else {
         const int wq = warp & 3, et = threadIdx.x - 64;

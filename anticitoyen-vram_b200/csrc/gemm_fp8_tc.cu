@@ -165,45 +165,54 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     pdl_launch_dependents();
 
     if (warp == 0) {
-        if (lane == 0) {
-            const uint32_t lead_full0 = cluster_map(full0, 0);
-            const CUtensorMap* weights = GATED && rank == 1 ? &map_w2 : &map_w;
-            auto load_w = [&](uint32_t dst, uint32_t bar, int kb, int tb) {
-                tma_load_2d_pair(dst, weights, bar, kb * FT_ROWS, GATED ? tb * FT_ROWS : tb * 2 * FT_ROWS + (int)rank * FT_ROWS);
-            };
-            int early = 0, asked = 0;
-            if (p.early_w && pair < n_items) {
-                int ta, tb;
-                ft_tile_of(pair, p.tiles_m, p.tiles_n, p.group, ta, tb);
-                early = min(STAGES, p.n_kb);
+        const uint32_t lead_full0 = cluster_map(full0, 0);
+        const CUtensorMap* weights = GATED && rank == 1 ? &map_w2 : &map_w;
+        auto load_w = [&](int s, int kb, int tb) {
+            tma_load_2d_pair(tiles_addr + s * FP_STAGE + FT_TILE, weights, lead_full0 + 8 * s, kb * FT_ROWS,
+                             GATED ? tb * FT_ROWS : tb * 2 * FT_ROWS + (int)rank * FT_ROWS);
+        };
+        int early = 0, asked = 0;
+        if (p.early_w && pair < n_items) {
+            int ta, tb;
+            ft_tile_of(pair, p.tiles_m, p.tiles_n, p.group, ta, tb);
+            early = min(STAGES, p.n_kb);
+            if (ft_elect()) {
                 for (int i = 0; i < early; ++i) {
                     if (rank == 0) mbar_expect_tx(full0 + 8 * i, 2 * FP_STAGE);
-                    load_w(tiles_addr + i * FP_STAGE + FT_TILE, lead_full0 + 8 * i, i, tb);
+                    load_w(i, i, tb);
                 }
             }
-            pdl_wait();
-            int s = 0;
-            uint32_t ph = 0;
-            for (int item = pair; item < n_items && !abort_s; item += n_pairs) {
-                int ta, tb;
-                ft_tile_of(item, p.tiles_m, p.tiles_n, p.group, ta, tb);
-                for (int kb = 0; kb < p.n_kb; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                    const uint32_t dst = tiles_addr + s * FP_STAGE;
-                    const bool half_done = early > 0;
-                    if (half_done) {
-                        --early;
-                    } else {
-                        if (!mbar_wait(empty0 + 8 * s, ph ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 1); break; }
-                        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * FP_STAGE);
-                    }
-                    ++asked;
-                    if (kb == p.skip_kb) continue;
-                    tma_load_2d_pair(dst, &map_x, lead_full0 + 8 * s, kb * FT_ROWS, ta * 2 * FT_ROWS + (int)rank * FT_ROWS);
-                    if (!half_done) load_w(dst + FT_TILE, lead_full0 + 8 * s, kb, tb);
-                }
-            }
-            if (abort_s && rank == 0) ft_drain(full0, STAGES, asked, p.wait_limit);
+            __syncwarp();
         }
+        pdl_wait();
+        int s = 0;
+        uint32_t ph = 0;
+        bool failed = false, ready = false;
+        for (int item = pair; item < n_items && !failed; item += n_pairs) {
+            int ta, tb;
+            ft_tile_of(item, p.tiles_m, p.tiles_n, p.group, ta, tb);
+            const int row = ta * 2 * FT_ROWS + (int)rank * FT_ROWS;
+#pragma unroll 1
+            for (int kb = 0; kb < p.n_kb; ++kb) {
+                const bool half_done = asked < early;
+                if (!half_done && !ready) {
+                    failed = ft_warp_failed(empty0 + 8 * s, ph ^ 1, &abort_s, p, 1);
+                    if (failed) break;
+                }
+                if (ft_elect()) {
+                    if (!half_done && rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * FP_STAGE);
+                    if (kb != p.skip_kb) {
+                        tma_load_2d_pair(tiles_addr + s * FP_STAGE, &map_x, lead_full0 + 8 * s, kb * FT_ROWS, row);
+                        if (!half_done) load_w(s, kb, tb);
+                    }
+                }
+                __syncwarp();
+                ++asked;
+                if (++s == STAGES) { s = 0; ph ^= 1; }
+                ready = __all_sync(0xffffffffu, ft_ready(empty0 + 8 * s, ph ^ 1));
+            }
+        }
+        if (failed && rank == 0) ft_drain(full0, STAGES, asked, p.wait_limit);
     } else if (warp == 1) {
         if (rank == 0) {
             pdl_wait();         // (the first tokens come after it: the wait for them starts there)
@@ -211,11 +220,11 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             const uint64_t a0 = umma_desc(tiles_addr), b0 = umma_desc(tiles_addr + FT_TILE);
             uint32_t turn = 0, ph = 0;
             int s = 0;
-            bool failed = false;
+            bool failed = false, ready = false;
             for (int item = pair; item < n_items && !failed; item += n_pairs) {
                 for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
                     const uint32_t slot = turn % FP_SLOTS, use = turn / FP_SLOTS;
-                    failed = ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3) || ft_warp_failed(tempty0 + 8 * slot, (use & 1) ^ 1, &abort_s, p, 2);
+                    failed = (!ready && ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) || ft_warp_failed(tempty0 + 8 * slot, (use & 1) ^ 1, &abort_s, p, 2);
                     if (failed) break;
                     tc_fence_after();
                     if (ft_elect()) {
@@ -228,6 +237,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                     }
                     __syncwarp();
                     if (++s == STAGES) { s = 0; ph ^= 1; }
+                    ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));       // (the next k-block has landed)
                 }
             }
         }
@@ -377,47 +387,60 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     pdl_launch_dependents();
     const int row_here = ta * FT_ROWS;
 
+    const int count = kb1 - kb0;
     if (warp == 0) {
-        if (lane == 0) {
-            auto load_w = [&](int s, int kb) {
-                const uint32_t dst = tiles_addr + s * S::STAGE + FT_TILE;
-                if (GATED) {
-                    tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS);
-                    tma_load_2d(dst + FT_TILE, &map_w2, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS);
-                } else {
-                    tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * BN);
-                }
-            };
-            const int early = p.early_w ? min(STAGES, kb1 - kb0) : 0;
+        auto load_w = [&](int s, int kb) {
+            const uint32_t dst = tiles_addr + s * S::STAGE + FT_TILE;
+            if (GATED) {
+                tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS);
+                tma_load_2d(dst + FT_TILE, &map_w2, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS);
+            } else {
+                tma_load_2d(dst, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * BN);
+            }
+        };
+        const int early = p.early_w ? min(STAGES, count) : 0;
+        if (ft_elect()) {
             for (int i = 0; i < early; ++i) {
                 mbar_expect_tx(full0 + 8 * i, S::STAGE);
                 load_w(i, kb0 + i);
             }
-            pdl_wait();
-            int s = 0, asked = 0;
-            uint32_t ph = 0;
-            for (int kb = kb0; kb < kb1; ++kb, s = (s + 1 == STAGES ? 0 : s + 1), ph ^= (s == 0)) {
-                const bool half_done = kb - kb0 < early;
-                if (!half_done) {
-                    if (!mbar_wait(empty0 + 8 * s, ph ^ 1, &abort_s, p.wait_limit)) { abort_s = 1; atomicExch(p.status, 1); break; }
-                    mbar_expect_tx(full0 + 8 * s, S::STAGE);
-                }
-                ++asked;
-                if (kb == p.skip_kb) continue;
-                tma_load_2d(tiles_addr + s * S::STAGE, &map_x, full0 + 8 * s, kb * FT_ROWS, row_here);
-                if (!half_done) load_w(s, kb);
-            }
-            if (abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
         }
+        __syncwarp();
+        pdl_wait();
+        int s = 0, asked = 0;
+        uint32_t ph = 0;
+        bool failed = false, ready = false;
+        for (; asked < count; ++asked) {
+            const bool half_done = asked < early;
+            const int kb = kb0 + asked;
+            if (!half_done && !ready) {
+                failed = ft_warp_failed(empty0 + 8 * s, ph ^ 1, &abort_s, p, 1);
+                if (failed) break;
+            }
+            if (ft_elect()) {
+                if (!half_done) mbar_expect_tx(full0 + 8 * s, S::STAGE);
+                if (kb != p.skip_kb) {
+                    tma_load_2d(tiles_addr + s * S::STAGE, &map_x, full0 + 8 * s, kb * FT_ROWS, row_here);
+                    if (!half_done) load_w(s, kb);
+                }
+            }
+            __syncwarp();
+            if (++s == STAGES) { s = 0; ph ^= 1; }
+            ready = __all_sync(0xffffffffu, ft_ready(empty0 + 8 * s, ph ^ 1));
+        }
+        if (failed || abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
     } else if (warp == 1) {
         pdl_wait();
         const uint32_t idesc = ft_idesc(BN, FT_ROWS);
         const uint64_t a0 = umma_desc(tiles_addr), b0 = umma_desc(tiles_addr + FT_TILE);
-        uint32_t turn = 0, ph = 0;
+        uint32_t ph = 0;
         int s = 0;
-        for (int kb = kb0; kb < kb1; ++kb, ++turn) {
-            const uint32_t buf = turn % S::SLOTS, use = turn / S::SLOTS;
-            if (ft_warp_failed(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p, 2) || ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) break;
+        bool ready = false;
+        for (int turn = 0; turn < count; ++turn) {
+            const uint32_t buf = (uint32_t)turn % S::SLOTS, use = (uint32_t)turn / S::SLOTS;
+            if ((!ready && ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) ||
+                (use && ft_warp_failed(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p, 2)))
+                break;
             tc_fence_after();
             if (ft_elect()) {
                 const uint64_t a = a0 + (uint64_t)(s * (S::STAGE >> 4)), b = b0 + (uint64_t)(s * (S::STAGE >> 4));
@@ -429,6 +452,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             }
             __syncwarp();
             if (++s == STAGES) { s = 0; ph ^= 1; }
+            ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));
         }
     } else {
         const int wq = warp & 3, part = (warp - 2) >> 2;
@@ -437,26 +461,25 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const int r = wq * 32 + lane;
         const float* sx = p.sx + (size_t)min(row_here + r, p.M - 1) * p.ldsx;
         const int block = GATED ? tb : min(tb * BN / FT_ROWS, (p.N - 1) / FT_ROWS);
-        const float *sw = p.sw + (size_t)block * p.ldsw, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : nullptr;
+        const float *sw = p.sw + (size_t)block * p.ldsw + kb0, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 + kb0 : nullptr;
         uint64_t sums[S::COLS / 2];
 #pragma unroll
         for (int i = 0; i < S::COLS / 2; ++i) sums[i] = 0;
         FtRowScales xs;
-        xs.begin(sx + kb0, kb1 - kb0, p.sx_vec && !(kb0 & 3));
-        float next_w = sw[kb0], next_w2 = GATED ? sw2[kb0] : 0.f;
-        uint32_t turn = 0;
-        for (int kb = kb0; kb < kb1; ++kb, ++turn) {
-            const float a = xs.take((int)turn), b = next_w, b2 = next_w2;
-            if (kb + 1 < kb1) {
-                next_w = sw[kb + 1];
-                if (GATED) next_w2 = sw2[kb + 1];
+        xs.begin(sx + kb0, count, p.sx_vec && !(kb0 & 3));
+        float next_w = sw[0], next_w2 = GATED ? sw2[0] : 0.f;
+        for (int turn = 0; turn < count; ++turn) {
+            const float x = xs.take(turn), s1 = x * next_w, s2 = GATED ? x * next_w2 : s1;
+            if (turn + 1 < count) {
+                next_w = sw[turn + 1];
+                if (GATED) next_w2 = sw2[turn + 1];
             }
-            const uint32_t buf = turn % S::SLOTS, use = turn / S::SLOTS;
+            const uint32_t buf = (uint32_t)turn % S::SLOTS, use = (uint32_t)turn / S::SLOTS;
             if (ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p)) break;
             tc_fence_after();
             const uint32_t t = taddr + buf * BN;
-            if (GATED) ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + FT_ROWS + part * 64, a * b, a * b2);
-            else ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + part * 64 + 32, a * b, a * b);
+            if (GATED) ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + FT_ROWS + part * 64, s1, s2);
+            else ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + part * 64 + 32, s1, s1);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(tempty0 + 8 * buf);
