@@ -147,7 +147,7 @@ __device__ __forceinline__ void ft_emit(const Fp8TcParams& p, uint32_t at, int l
                 if (r + j * step >= rows) break;
                 const size_t row = (size_t)(row0 + r + j * step);
                 const float4 g = gs[j], u = us[j];
-                const float h[4] = {silu_f32<float>(g.x) * u.x, silu_f32<float>(g.y) * u.y, silu_f32<float>(g.z) * u.z, silu_f32<float>(g.w) * u.w};
+                const float h[4] = {fp8_silu(g.x) * u.x, fp8_silu(g.y) * u.y, fp8_silu(g.z) * u.z, fp8_silu(g.w) * u.w};
                 uint32_t m = max(max(fp8_magnitude(h[0]), fp8_magnitude(h[1])), max(fp8_magnitude(h[2]), fp8_magnitude(h[3])));
                 m = __reduce_max_sync(0xffffffffu, m);
                 const Fp8Scale k = fp8_scale(m);

@@ -22,46 +22,26 @@ struct GnParams {
     float c, e1, e2, inv_h;
 };
 
+// XT, DT: the stream's and the part's element type, 0 bfloat16, 1 float, 2 as the parameters say (a type known when the kernel is built
+// halves what a row costs in instructions, which is what bounds many rows beside memory)
+template <int TYPE>
+__device__ __forceinline__ int gn_f32(int said) { return TYPE == 2 ? said : TYPE; }
 template <bool VEC>
 __device__ __forceinline__ void gn_load(const void* row, int f32, int at, int H, float (&v)[8]) {
     if (VEC) raw8_floats(raw8_load(row, f32, at), f32, v);
     else load8_ragged(row, f32, at, H, v);
 }
 
-// C: pieces of eight elements a thread.  With one piece the weights fit the registers beside it and are asked for early; with more
-// they are read where they are used.
-template <bool VEC, int C>
-__global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
-    __shared__ float red[32];
-    pdl_launch_dependents();
-    const int H = p.H;
-    float w1[8], w2[8], gc[8];
-    if (C == 1) {
-        const int at = threadIdx.x * 8;
-        if (at < H) {
-            if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
-            if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
-            if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
-        }
-    }
-    pdl_wait();
-    const size_t row = blockIdx.x;
-    char* xr = reinterpret_cast<char*>(p.x) + row * p.ldx * (p.x_f32 ? 4 : 2);
-    const char* dr = reinterpret_cast<const char*>(p.d) + row * p.ldd * (p.d_f32 ? 4 : 2);
+// A row whose pieces are in `xw`, `dw` and `gw` (VEC), or are read here element by element.  C: pieces of eight elements a thread; with
+// one the weights are in `w1`, `w2` and `gc` already, with more they are read where they are used.
+template <bool VEC, int C, int XT, int DT>
+__device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8 (&xw)[C], const Raw8 (&dw)[C], const Raw8 (&gw)[C],
+                                       float (&w1)[8], float (&w2)[8], float (&gc)[8], float* red) {
+    const int H = p.H, x_f32 = gn_f32<XT>(p.x_f32), d_f32 = gn_f32<DT>(p.d_f32);
+    char* xr = reinterpret_cast<char*>(p.x) + row * p.ldx * (x_f32 ? 4 : 2);
+    const char* dr = reinterpret_cast<const char*>(p.d) + row * p.ldd * (d_f32 ? 4 : 2);
     const char* gr = p.g ? reinterpret_cast<const char*>(p.g) + row * p.ldg * (p.g_f32 ? 4 : 2) : nullptr;
-    Raw8 xw[C], dw[C], gw[C];
     float x[C][8], d[C][8];
-    if (VEC) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-            const int at = (threadIdx.x + i * blockDim.x) * 8;
-            if (at < H) {
-                if (p.d) dw[i] = raw8_load(dr, p.d_f32, at);
-                xw[i] = raw8_load(xr, p.x_f32, at);
-                if (gr) gw[i] = raw8_load(gr, p.g_f32, at);
-            }
-        }
-    }
     if (p.d) {
         float r = 1.f;
         if (p.w1) {
@@ -70,8 +50,8 @@ __global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
             for (int i = 0; i < C; ++i) {
                 const int at = (threadIdx.x + i * blockDim.x) * 8;
                 if (at < H) {
-                    if (VEC) raw8_floats(dw[i], p.d_f32, d[i]);
-                    else load8_ragged(dr, p.d_f32, at, H, d[i]);
+                    if (VEC) raw8_floats(dw[i], d_f32, d[i]);
+                    else load8_ragged(dr, d_f32, at, H, d[i]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ss = fmaf(d[i][e], d[i][e], ss);
                 }
@@ -88,13 +68,14 @@ __global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[i][e] = d[i][e] * r * w1[e];
             } else {
-                if (VEC) raw8_floats(dw[i], p.d_f32, d[i]);
-                else load8_ragged(dr, p.d_f32, at, H, d[i]);
+                if (VEC) raw8_floats(dw[i], d_f32, d[i]);
+                else load8_ragged(dr, d_f32, at, H, d[i]);
             }
             if (gr) {
                 float g[8];
-                if (VEC) raw8_floats(gw[i], p.g_f32, g);
-                else load8_ragged(gr, p.g_f32, at, H, g);
+                if (!VEC) load8_ragged(gr, p.g_f32, at, H, g);
+                else if (p.g_f32) raw8_floats(gw[i], 1, g);
+                else raw8_floats(gw[i], 0, g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[i][e] *= g[e];
             } else if (p.gc) {
@@ -102,23 +83,23 @@ __global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) d[i][e] *= gc[e];
             }
-            if (VEC) raw8_floats(xw[i], p.x_f32, x[i]);
-            else load8_ragged(xr, p.x_f32, at, H, x[i]);
+            if (VEC) raw8_floats(xw[i], x_f32, x[i]);
+            else load8_ragged(xr, x_f32, at, H, x[i]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 x[i][e] = fmaf(p.c, d[i][e], x[i][e]);
-                if (!p.x_f32) x[i][e] = round_to<bf16>(x[i][e]);
+                if (!x_f32) x[i][e] = round_to<bf16>(x[i][e]);
             }
-            if (VEC) store8(xr, p.x_f32, at, x[i]);
-            else store8_ragged(xr, p.x_f32, at, H, x[i]);
+            if (VEC) store8(xr, x_f32, at, x[i]);
+            else store8_ragged(xr, x_f32, at, H, x[i]);
         }
     } else {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             const int at = (threadIdx.x + i * blockDim.x) * 8;
             if (at >= H) continue;
-            if (VEC) raw8_floats(xw[i], p.x_f32, x[i]);
-            else load8_ragged(xr, p.x_f32, at, H, x[i]);
+            if (VEC) raw8_floats(xw[i], x_f32, x[i]);
+            else load8_ragged(xr, x_f32, at, H, x[i]);
         }
     }
     if (p.out_kind == 3) return;
@@ -161,17 +142,53 @@ __global__ void __launch_bounds__(512) gated_norms_kernel(const GnParams p) {
     }
 }
 
+// A block a row.  BLOCKS of 512 threads have to fit an SM: 2 holds a thread to 64 registers.
+template <bool VEC, int C, int XT, int DT, int BLOCKS>
+__global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams p) {
+    __shared__ float red[32];
+    pdl_launch_dependents();
+    const int H = p.H;
+    float w1[8], w2[8], gc[8];
+    if (C == 1) {
+        const int at = threadIdx.x * 8;
+        if (at < H) {
+            if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
+            if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
+            if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
+        }
+    }
+    pdl_wait();
+    const size_t row = blockIdx.x;
+    Raw8 xw[C], dw[C], gw[C];
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            if (at < H) {
+                const int x_f32 = gn_f32<XT>(p.x_f32), d_f32 = gn_f32<DT>(p.d_f32);
+                if (p.d) dw[i] = raw8_load(reinterpret_cast<const char*>(p.d) + row * p.ldd * (d_f32 ? 4 : 2), d_f32, at);
+                xw[i] = raw8_load(reinterpret_cast<const char*>(p.x) + row * p.ldx * (x_f32 ? 4 : 2), x_f32, at);
+                if (p.g) gw[i] = raw8_load(reinterpret_cast<const char*>(p.g) + row * p.ldg * (p.g_f32 ? 4 : 2), p.g_f32, at);
+            }
+        }
+    }
+    gn_row<VEC, C, XT, DT>(p, row, xw, dw, gw, w1, w2, gc, red);
+}
+
 // Pieces of eight elements a thread: with few rows one as long as 512 threads cover a row, for a row's time is then its chain of loads,
-// sums and stores, and more warps bring it in sooner; with many rows four, so that more rows are under way on an SM and what a warp does
-// once for a row serves more of it (4096 rows of 4096, bfloat16 in, e4m3 out: 64 us with one piece, GN_MANY with four).
-template <bool VEC>
+// sums and stores, and more warps bring it in sooner (150 rows of 5120 with one, two and two pieces at 64 registers: -, 4.8, 5.6 us; 300 of
+// 4096: 3.7, 3.9, 3.9).  With many rows two, and as many blocks to an SM as 64 registers allow: what a warp does once for a row (sums over
+// the block, the scales' divisions) serves more of it, and what is left of a row's time are its instructions (4096 rows of 4096, bfloat16 in,
+// e4m3 out, with one, two and four pieces 34, 26, 32 us; of 5120, a float stream and a gate for every token 55, 49, 53, of which 45 is memory's).
+template <bool VEC, int XT, int DT>
 static int gn_launch(const GnParams& p, int T, int sms, cudaStream_t stream) {
     const int pieces = (p.H + 7) / 8;
     auto threads = [&](int c) { return ((pieces + c - 1) / c + 31) / 32 * 32; };
     const bool few = T <= 2 * sms;
-    if (few && threads(1) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 1>, T, threads(1), 0, stream, p);
-    else if (few && threads(2) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 2>, T, threads(2), 0, stream, p);
-    else if (threads(4) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 4>, T, threads(4), 0, stream, p);
+    if (few && threads(1) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 1, XT, DT, 1>, T, threads(1), 0, stream, p);
+    else if (few && threads(2) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 2, XT, DT, 1>, T, threads(2), 0, stream, p);
+    else if (threads(2) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 2, XT, DT, 2>, T, threads(2), 0, stream, p);
+    else if (threads(4) <= 512) acv_launch(PDL_NORM, gated_norms_kernel<VEC, 4, XT, DT, 1>, T, threads(4), 0, stream, p);
     else return ACV_ERR_SIZE;
     return acv_launch_status();
 }
@@ -203,5 +220,7 @@ ACV_API int acv_add_gated_norms(const GatedNormsArgs* a) {
                      (p.out_kind == 3 || fp8_rows_aligned(p.out, p.ldo, ob, p.out_kind == 2 ? 8 : 16)) &&
                      !(((uintptr_t)p.gc | (uintptr_t)p.w1 | (uintptr_t)p.w2) & 15);
     const cudaStream_t stream = (cudaStream_t)const_cast<void*>(a->stream);
-    return vec ? gn_launch<true>(p, T, a->sms, stream) : gn_launch<false>(p, T, a->sms, stream);
+    if (!vec) return gn_launch<false, 2, 2>(p, T, a->sms, stream);
+    if (p.x_f32) return p.d_f32 ? gn_launch<true, 1, 1>(p, T, a->sms, stream) : gn_launch<true, 1, 0>(p, T, a->sms, stream);
+    return p.d_f32 ? gn_launch<true, 0, 1>(p, T, a->sms, stream) : gn_launch<true, 0, 0>(p, T, a->sms, stream);
 }

@@ -40,8 +40,7 @@ __device__ __forceinline__ void ft_add_tile(uint64_t* sums, uint32_t first, uint
     }
 }
 
-// A row's scales, four k-blocks at a time and four ahead of their use: lanes hold rows, so a load touches 32 lines whatever its width
-// (one number at a time, those lookups took 1000 cycles a k-block, twice what the tensor core needs).
+// A row's scales, four k-blocks at a time and four ahead of their use: lanes hold rows, so a load looks 32 lines up whatever its width.
 struct FtRowScales {
     const float* at;
     int left, vec;
@@ -293,7 +292,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
                     const float2 g = ft_floats(sums[i]), u = ft_floats(sums[32 + i]);
-                    const float a = silu_f32<float>(g.x) * u.x, b = silu_f32<float>(g.y) * u.y;
+                    const float a = fp8_silu(g.x) * u.x, b = fp8_silu(g.y) * u.y;
                     m = max(m, max(fp8_magnitude(a), fp8_magnitude(b)));
                     sums[i] = ft_pair(a, b);
                 }
@@ -387,7 +386,10 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     pdl_launch_dependents();
     const int row_here = ta * FT_ROWS;
 
-    const int count = kb1 - kb0;
+    // Each column of tiles begins at another of its k-blocks (a multiple of four) and goes round: the CTAs, which start together, would
+    // all read the same tokens' bytes at the same time (a tile's order is its own, whatever the others do).
+    const int count = kb1 - kb0, turned = (int)((unsigned)tb * 20u % (unsigned)count) & ~3, wrap = count - turned;
+    auto block_of = [&](int i) { return i < wrap ? i + turned : i - wrap; };
     if (warp == 0) {
         auto load_w = [&](int s, int kb) {
             const uint32_t dst = tiles_addr + s * S::STAGE + FT_TILE;
@@ -402,7 +404,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         if (ft_elect()) {
             for (int i = 0; i < early; ++i) {
                 mbar_expect_tx(full0 + 8 * i, S::STAGE);
-                load_w(i, kb0 + i);
+                load_w(i, kb0 + block_of(i));
             }
         }
         __syncwarp();
@@ -412,7 +414,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         bool failed = false, ready = false;
         for (; asked < count; ++asked) {
             const bool half_done = asked < early;
-            const int kb = kb0 + asked;
+            const int kb = kb0 + block_of(asked);
             if (!half_done && !ready) {
                 failed = ft_warp_failed(empty0 + 8 * s, ph ^ 1, &abort_s, p, 1);
                 if (failed) break;
@@ -466,13 +468,14 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 #pragma unroll
         for (int i = 0; i < S::COLS / 2; ++i) sums[i] = 0;
         FtRowScales xs;
-        xs.begin(sx + kb0, count, p.sx_vec && !(kb0 & 3));
-        float next_w = sw[0], next_w2 = GATED ? sw2[0] : 0.f;
+        xs.begin(sx + kb0 + turned, wrap, p.sx_vec && !(kb0 & 3));
+        float next_w = sw[turned], next_w2 = GATED ? sw2[turned] : 0.f;
         for (int turn = 0; turn < count; ++turn) {
-            const float x = xs.take(turn), s1 = x * next_w, s2 = GATED ? x * next_w2 : s1;
+            if (turn == wrap) xs.begin(sx + kb0, turned, p.sx_vec && !(kb0 & 3));
+            const float x = xs.take(turn < wrap ? turn : turn - wrap), s1 = x * next_w, s2 = GATED ? x * next_w2 : s1;
             if (turn + 1 < count) {
-                next_w = sw[turn + 1];
-                if (GATED) next_w2 = sw2[turn + 1];
+                next_w = sw[block_of(turn + 1)];
+                if (GATED) next_w2 = sw2[block_of(turn + 1)];
             }
             const uint32_t buf = (uint32_t)turn % S::SLOTS, use = (uint32_t)turn / S::SLOTS;
             if (ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p)) break;
