@@ -49,14 +49,6 @@ __device__ __forceinline__ void ft_wait_ld(uint32_t (&r)[16]) {
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
                    "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
-__device__ __forceinline__ void ft_wait_ld2(uint32_t (&r)[32], uint32_t (&q)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i += 8)
-        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]),
-                          "+r"(q[i]), "+r"(q[i + 1]), "+r"(q[i + 2]), "+r"(q[i + 3]), "+r"(q[i + 4]), "+r"(q[i + 5]), "+r"(q[i + 6]), "+r"(q[i + 7])
-                     ::"memory");
-}
 __device__ __forceinline__ void ft_fma2(uint64_t& sum, uint32_t lo, uint32_t hi, uint64_t scale) {
     asm("{\n\t.reg .b64 v;\n\tmov.b64 v, {%1, %2};\n\tfma.rn.f32x2 %0, v, %3, %0;\n\t}" : "+l"(sum) : "r"(lo), "r"(hi), "l"(scale));
 }

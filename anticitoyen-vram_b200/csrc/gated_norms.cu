@@ -7,8 +7,7 @@
 // h is rounded once, to float, bfloat16, or e4m3 with a scale for each group of 128 (fp8.cuh), which is what an 8-bit product reads.
 // One block a row; a thread keeps its elements (eight neighbouring ones, C such pieces) in registers from their only read to their
 // only write, both statistics are 32-bit sums over the block.  Sixteen neighbouring lanes hold a group, so its maximum takes four
-// exchanges.  Memory bounds it with many rows, the chain load - sum - sum - store with few; the weights, which no kernel before
-// this one writes, are asked for before the wait for that kernel.
+// exchanges.  Memory bounds it with many rows, the chain load - sum - sum - store with few.
 #include "fp8.cuh"
 
 struct GnParams {
@@ -148,15 +147,6 @@ __global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams
     __shared__ float red[32];
     pdl_launch_dependents();
     const int H = p.H;
-    float w1[8], w2[8], gc[8];
-    if (C == 1) {
-        const int at = threadIdx.x * 8;
-        if (at < H) {
-            if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
-            if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
-            if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
-        }
-    }
     pdl_wait();
     const size_t row = blockIdx.x;
     Raw8 xw[C], dw[C], gw[C];
@@ -170,6 +160,15 @@ __global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams
                 xw[i] = raw8_load(reinterpret_cast<const char*>(p.x) + row * p.ldx * (x_f32 ? 4 : 2), x_f32, at);
                 if (p.g) gw[i] = raw8_load(reinterpret_cast<const char*>(p.g) + row * p.ldg * (p.g_f32 ? 4 : 2), p.g_f32, at);
             }
+        }
+    }
+    float w1[8], w2[8], gc[8];
+    if (C == 1) {
+        const int at = threadIdx.x * 8;
+        if (at < H) {
+            if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
+            if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
+            if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
         }
     }
     gn_row<VEC, C, XT, DT>(p, row, xw, dw, gw, w1, w2, gc, red);

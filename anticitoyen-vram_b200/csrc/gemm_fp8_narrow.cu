@@ -190,17 +190,18 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             }
         }
     }
+    // (tensor memory goes back before the cluster's CTAs wait for one another, see gemm_fp8_tc.cu)
     tc_fence_before();
-    if (size > 1) cluster_sync_all();
-    else __syncthreads();
-    if (!abort_s)
-        ft_emit<FT_ROWS, GATED, HALVES, 1>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
-    // (the peers may still read this CTA's sums)
-    if (size > 1) cluster_sync_all();
+    __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }
+    if (size > 1) cluster_sync_all();
+    if (!abort_s)
+        ft_emit<FT_ROWS, GATED, HALVES, 1>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
+    // (the peers may still read this CTA's sums)
+    if (size > 1) cluster_sync_all();
 }
 
 template <int BT, bool GATED>

@@ -499,17 +499,19 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             }
         }
     }
+    // Tensor memory goes back before the cluster's CTAs wait for one another: a CTA that held some while it waited for a peer, which waits for
+    // some that another kernel's CTA holds in the same way, would wait for good.
     tc_fence_before();
-    if (p.splits > 1) cluster_sync_all();
-    else __syncthreads();
-    if (!abort_s)
-        ft_emit<BN, GATED, 1, 2>(p, tiles_addr, S::LD, split + p.splits * warp, p.splits * (S::THREADS / 32), min(FT_ROWS, p.M - row_here), row_here, tb);
-    // (the peers may still read this CTA's sums)
-    if (p.splits > 1) cluster_sync_all();
+    __syncthreads();
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }
+    if (p.splits > 1) cluster_sync_all();
+    if (!abort_s)
+        ft_emit<BN, GATED, 1, 2>(p, tiles_addr, S::LD, split + p.splits * warp, p.splits * (S::THREADS / 32), min(FT_ROWS, p.M - row_here), row_here, tb);
+    // (the peers may still read this CTA's sums)
+    if (p.splits > 1) cluster_sync_all();
 }
 
 // ----------------------------------------------------------------------------- host side
@@ -596,7 +598,8 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
 //   Splits of K are what fits the SMs at once in clusters, two CTAs of kind 4 to an SM (three of the gated form, whose cluster holds two
 // halves of a group), one of kind 2, and at least four k-blocks to each: 16 tokens 6144 x 4096 in 2, 4, 6 splits 7.9, 6.1, 9.8; 4096 x 1024
 // in 1, 2, 4: 4.3, 3.8, 4.2; 12288 units, K 4096, in 1, 2, 3: 21.0, 19.2, 24.8; kind 2, 65 tokens 4096 x 12288 in 2, 3, 4, 6: 19.5, 15.9,
-// 14.0, 23.3.
+// 14.0, 23.3.  Kind 4 holds the scales of its k-blocks in shared memory beside its stages: 160 KB of them at most, about 80 thousand k to a
+// split of 32 tokens' gated form, and longer rows are kind 2's (one that holds none).
 //   Pairs of CTAs and tiles of 128 rows both come in rounds over the SMs, and a round of pairs takes 1.3 of a round of tiles of 128 x 128,
 // 0.83 of one of gated tiles of 128 x 256 (K 4096: 16.2 us, 21; 37.5, 31.2): 512 tokens 4096 x 4096 16.2 and 19.8, 6144 x 4096 32.1 and 22.5,
 // 384 tokens of 12288 units 76 and 93, 512 of them 113 and 94.
@@ -610,7 +613,9 @@ static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
         if (gated) splits = wide <= 3 * fit(4) && n_kb >= 4 ? 2 : 1;
         else
             while (splits < 8 && wide <= 2 * fit(splits + 1) && n_kb >= 4 * (splits + 1)) ++splits;
-        return {4, M <= 16 ? 16 : 32, splits};
+        const int bt = M <= 16 ? 16 : 32;
+        if ((n_kb + splits - 1) / splits * (gated ? 2 : 1) * (bt + 1) * 4 <= 160 * 1024) return {4, bt, splits};
+        splits = 1;
     }
     const long long tiles = deep * wide, pairs = (deep + 1) / 2 * (gated ? wide : (wide + 1) / 2);
     const long long tile_rounds = (tiles + sms - 1) / sms, pair_rounds = (pairs + sms / 2 - 1) / (sms / 2);
@@ -622,7 +627,12 @@ static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
 static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cudaStream_t stream) {
     const bool gated = o.w2 != nullptr;
     if (o.M <= 0 || o.N <= 0) return 0;
-    if (o.K <= 0) return ACV_ERR_SIZE;
+    if (o.K <= 0 || max(o.M, max(o.N, o.K)) > 0x7fffffff - 1024) return ACV_ERR_SIZE;       // (sizes are rounded up to tiles in 32 bits)
+    // a single row's stride says nothing; several rows do not overlap
+    const long long row_bytes = ((long long)o.K + 15) / 16 * 16;
+    if (o.M == 1) o.ldx = row_bytes;
+    if (o.N == 1) { o.ldw = row_bytes; if (gated) o.ldw2 = row_bytes; }
+    if (o.ldx < o.K || o.ldw < o.K || (gated && o.ldw2 < o.K)) return ACV_ERR_ALIGN;
     if (((uintptr_t)o.x | (uintptr_t)o.w | (uintptr_t)o.w2) % 16 || (o.ldx | o.ldw | o.ldw2) % 16) return ACV_ERR_ALIGN;
     const Fp8Plan how = plan ? Fp8Plan{plan & 15, (plan >> 4) & 0xfff, plan >> 16} : ft_plan(o.M, o.N, o.K, gated, sms);
     if (how.kind == 1) return acv_fp8_rows(o, flags, stream);

@@ -113,6 +113,7 @@ ACV_API int acv_quantize_fp8(const QuantizeFp8Args* a) {
     const int dtype = a->dtype, T = a->T, K = a->K, block_rows = a->block_rows, sms = a->sms;
     const cudaStream_t stream = (cudaStream_t)const_cast<void*>(a->stream);
     if (T <= 0 || K <= 0) return 0;
+    if (K > 0x7fffffff - 1024) return ACV_ERR_SIZE;         // (rounded up to groups in 32 bits)
     if (dtype != ACV_F32 && dtype != ACV_BF16) return ACV_ERR_DTYPE;
     const int f32 = dtype == ACV_F32;
     const int G = (K + FP8_GROUP - 1) / FP8_GROUP;

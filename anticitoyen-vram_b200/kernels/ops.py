@@ -2404,11 +2404,15 @@ def _launch_record(device: int, name: str, record: struct.Struct, at: int, *fiel
     entry = _entries.get(name)
     if entry is None:
         entry = _entries[name] = getattr(library(), "acv_" + name)
+    try:
+        packed = record.pack(*fields[:at], torch._C._cuda_getCurrentRawStream(device), *fields[at:])
+    except struct.error as e:
+        raise KernelError(f"{name}: {_ERRORS[-3]} ({e})") from None
     if device == torch._C._cuda_getDevice():
-        _check(entry(record.pack(*fields[:at], torch._C._cuda_getCurrentRawStream(device), *fields[at:])), name)
+        _check(entry(packed), name)
     else:
         with torch.cuda.device(device):
-            _check(entry(record.pack(*fields[:at], torch._C._cuda_getCurrentRawStream(device), *fields[at:])), name)
+            _check(entry(packed), name)
 
 
 def _sms_of(device: int) -> int:
@@ -2459,13 +2463,14 @@ def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, bl
 
 
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
-               plan: tuple | None = None) -> torch.Tensor:
+               static_weights: bool = False, plan: tuple | None = None) -> torch.Tensor:
     """out[T, N] = x @ w^T of quantised matrices: x [T, K] with a scale for each group of 128 of a row, w [N, K] with a scale for each
-    block of 128 x 128; out float32 or bfloat16, dense rows at any stride.  A group's sum is multiplied by its two scales in float
-    and joins a float sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``).
+    block of 128 x 128; out float32 or bfloat16, dense rows at any stride.  A group's sum is multiplied by its two scales' float
+    product and joins a float sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``) and do not overlap.
 
-    The weights are read while the kernel in front of this one may still run: they were written long before.  ``plan``: (kind, columns
-    of a tile, splits of K) as csrc/gemm_fp8_tc.cu names them, in place of its own choice."""
+    ``static_weights``: w and its scales were written long before this call (a model's weights), so the kernel may read them while
+    the kernels before it in the stream are still running.  ``plan``: (kind, columns of a tile, splits of K) as csrc/gemm_fp8_tc.cu
+    names them, in place of its own choice."""
     T, K = x.shape
     N, Kw = w.shape
     G = (K + 127) // 128
@@ -2485,15 +2490,16 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
         return out.zero_()
     _launch_record(device, "linear_fp8", _LINEAR_ARGS, 9, x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), out.data_ptr(),
                    0, 0, 0, _status_at.get(device) or _status_pointer(x) or 0, xs[0], xss[0], ws[0], wss[0], outs[0], 0, 0, 0, T, N, K,
-                   out.dtype is torch.float32, 1, 0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16, _sms_of(device))
+                   out.dtype is torch.float32, 1 if static_weights else 0, 0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16, _sms_of(device))
     return out
 
 
 def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tensor, gate_scales: torch.Tensor, up: torch.Tensor,
-                      up_scales: torch.Tensor, out: torch.Tensor, out_scales: torch.Tensor,
+                      up_scales: torch.Tensor, out: torch.Tensor, out_scales: torch.Tensor, static_weights: bool = False,
                       plan: tuple | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(out, out_scales) = silu(x @ gate^T) * (x @ up^T), quantised in groups of 128 units: what the next ``linear_fp8`` reads.
-    Operands as there, gate and up [I, K] each with its own scales.  Unit and quantisation are float, from the float sums."""
+    Operands, ``static_weights`` and ``plan`` as there, gate and up [I, K] each with its own scales.  Unit and quantisation are float,
+    from the float sums."""
     T, K = x.shape
     I, Kw = gate.shape
     G, B = (K + 127) // 128, (I + 127) // 128
@@ -2518,7 +2524,7 @@ def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tenso
         raise KernelError("linear_fp8_swiglu: K is 0")
     _launch_record(device, "linear_fp8", _LINEAR_ARGS, 9, x.data_ptr(), x_scales.data_ptr(), gate.data_ptr(), gate_scales.data_ptr(),
                    out.data_ptr(), up.data_ptr(), up_scales.data_ptr(), out_scales.data_ptr(), _status_at.get(device) or _status_pointer(x) or 0,
-                   xs[0], xss[0], gs[0], gss[0], outs[0], us[0], uss[0], outss[0], T, I, K, 0, 1,
+                   xs[0], xss[0], gs[0], gss[0], outs[0], us[0], uss[0], outss[0], T, I, K, 0, 1 if static_weights else 0,
                    0 if plan is None else plan[0] | plan[1] << 4 | plan[2] << 16, _sms_of(device))
     return out, out_scales
 

@@ -129,7 +129,8 @@ class SwiGLU(FeedForward):
         if self.fp8:
             h = Fp8Rows.of(h)
             act = Fp8Rows(h.shape[0], self.intermediate_size, h.device, h.dtype)
-            ops.linear_fp8_swiglu(h.values, h.scales, *self.gate.matrices[0], *self.up.matrices[0], act.values, act.scales)
+            ops.linear_fp8_swiglu(h.values, h.scales, *self.gate.matrices[0], *self.up.matrices[0], act.values, act.scales,
+                                  static_weights=True)
             return self.down(act)
         act = h.new_empty((h.shape[0], self.intermediate_size))
         self.inner(h, ctx, act)

@@ -169,9 +169,9 @@ class Fp8Linear:
         x = Fp8Rows.of(x)
         out = x.new_empty((x.shape[0], self.out_features), dtype=out_dtype or x.dtype)
         if len(self.matrices) == 1:
-            return ops.linear_fp8(x.values, x.scales, *self.matrices[0], out)
+            return ops.linear_fp8(x.values, x.scales, *self.matrices[0], out, static_weights=True)
         at = 0
         for values, scales in self.matrices:
-            ops.linear_fp8(x.values, x.scales, values, scales, out[:, at:at + values.shape[0]])
+            ops.linear_fp8(x.values, x.scales, values, scales, out[:, at:at + values.shape[0]], static_weights=True)
             at += values.shape[0]
         return out

@@ -323,3 +323,201 @@ def test_norms_of_rows_of_zeros():
     q, s = ops().fp8_rows(2, H, DEV)
     ops().add_gated_norms(x, d, q, s, post_weight=w, post_eps=1e-6, weight=w, eps=1e-6)
     assert bool((x == 0).all()) and bool((q.float() == 0).all()) and bool((s == 2.0 ** -126).all())
+
+
+# ----------------------------------------------------------------------------- calls one behind the other
+def chain(x, wide, T):
+    """Quantised weights, norm, gated product, product, as a step runs them, everything made by the kernel in front."""
+    o = ops()
+    H, I = x.shape[1], wide.shape[0]
+    g, gs = o.fp8_rows(I, H, DEV)[0], torch.empty((groups(I), groups(H)), device=DEV)
+    o.quantize_fp8(wide, g, gs, 128)
+    q, s = o.fp8_rows(T, H, DEV)
+    o.add_gated_norms(x, x.clone(), q, s, weight=torch.ones(H, device=DEV), eps=1e-6)
+    a, b = o.fp8_rows(T, I, DEV)
+    o.linear_fp8_swiglu(q, s, g, gs, g, gs, a, b)
+    d, ds = o.fp8_rows(H, I, DEV)[0], torch.empty((groups(H), groups(I)), device=DEV)
+    o.quantize_fp8(wide.t().contiguous(), d, ds, 128)
+    out = torch.empty((T, H), device=DEV)
+    o.linear_fp8(a, b, d, ds, out)
+    return [t.clone() for t in (q.view(torch.uint8), s, a.view(torch.uint8), b, out)]
+
+
+@pytest.mark.parametrize("T", [1, 16, 30, 100, 600])
+def test_a_chain_whose_every_input_is_made_by_the_kernel_in_front(T):
+    """Kernels begin while the one in front still runs: run without a pause the chain gives what it gives with a wait behind every call."""
+    H, I = 512, 1280
+    wide = (0.05 * activations(I, H, 3)).to(DEV)
+    x0 = activations(T, H, 4, BF).to(DEV)
+    import contextlib
+
+    @contextlib.contextmanager
+    def waiting():
+        o = ops()
+        real = o._launch_record
+        def launch(*args):
+            real(*args)
+            torch.cuda.synchronize()
+        o._launch_record = launch
+        try:
+            yield
+        finally:
+            o._launch_record = real
+
+    with waiting():
+        want = chain(x0.clone(), wide, T)
+    for _ in range(20):
+        for a, b in zip(chain(x0.clone(), wide, T), want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T", [1, 12, 40, 300])
+def test_captured_and_on_two_streams(T):
+    """Two captured graphs and two streams at once share nothing but the status word."""
+    K, N = 1024, 640
+    x, xs = quantized(T, K, 1, 1)
+    sets = []
+    for i in range(2):
+        w, ws = quantized(N, K, 2 + i, 128, 0.02)
+        u, us = quantized(N, K, 8 + i, 128, 0.02)
+        sets.append((w, ws, u, us))
+
+    def run(i):
+        w, ws, u, us = sets[i]
+        out = torch.empty((T, N), device=DEV)
+        ops().linear_fp8(x, xs, w, ws, out, static_weights=True)
+        q, s = ops().fp8_rows(T, N, DEV)
+        ops().linear_fp8_swiglu(x, xs, w, ws, u, us, q, s, static_weights=True)
+        return out, q.view(torch.uint8), s
+
+    want = [[t.clone() for t in run(i)] for i in range(2)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(run(i))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for i in (0, 1):
+            for t in outs[i]:
+                t.zero_() if t.dtype != torch.uint8 else t.fill_(0)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            for a, b in zip(outs[i], want[i]):
+                assert torch.equal(a, b)
+    for _ in range(10):
+        got = []
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append(run(i))
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            for a, b in zip(got[i], want[i]):
+                assert torch.equal(a, b)
+    assert ops().gemm_status() == 0
+
+
+# ----------------------------------------------------------------------------- the ends of the range
+def test_rows_that_are_not_on_16_bytes_are_refused():
+    x, xs = quantized(4, 256, 1, 1)
+    w, ws = quantized(8, 256, 2, 128)
+    out = torch.empty((4, 8), device=DEV)
+    flat = torch.zeros(4 * 264 + 1, dtype=torch.uint8, device=DEV).view(FP8)
+    for bad in (flat[:4 * 264].view(4, 264)[:, :256], flat[1:1 + 4 * 256].view(4, 256), x[:1].expand(4, 256), flat.as_strided((4, 256), (16, 1))):
+        with pytest.raises(ops().KernelError, match="aligned"):
+            ops().linear_fp8(bad, xs, w, ws, out)
+    bad = torch.zeros((8, 264), dtype=torch.uint8, device=DEV).view(FP8)[:, :256]
+    with pytest.raises(ops().KernelError, match="aligned"):
+        ops().linear_fp8(x, xs, bad, ws, out)
+    q, s = ops().fp8_rows(4, 8, DEV)
+    for g, u in ((w, bad), (bad, w)):
+        with pytest.raises(ops().KernelError, match="aligned"):
+            ops().linear_fp8_swiglu(x, xs, g, ws, u, ws, q, s)
+
+
+@pytest.mark.parametrize("plan", [None, (2, 128, 1), (4, 16, 1)])
+def test_a_single_row_has_no_stride(plan):
+    x, xs = quantized(3, 250, 1, 1)
+    w, ws = quantized(1, 250, 2, 128)
+    want = ops().linear_fp8(x[:1], xs[:1], w, ws, torch.empty((1, 1), device=DEV), plan=plan)
+    got = ops().linear_fp8(x[:1].clone(memory_format=torch.contiguous_format), xs[:1], w.as_strided((1, 250), (3, 1)), ws,
+                           torch.empty((1, 1), device=DEV), plan=plan)
+    assert torch.equal(want, got)
+
+
+def test_no_tokens_no_features_and_no_inner_elements():
+    e = lambda r, c, dt=F32: torch.empty((r, c), device=DEV, dtype=dt)
+    w, ws = quantized(8, 256, 2, 128)
+    assert ops().linear_fp8(e(0, 256, FP8), e(0, 2), w, ws, e(0, 8)).shape == (0, 8)
+    x, xs = quantized(4, 256, 1, 1)
+    assert ops().linear_fp8(x, xs, e(0, 256, FP8), e(0, 2), e(4, 0)).shape == (4, 0)
+    out = torch.full((4, 8), 5.0, device=DEV)
+    ops().linear_fp8(e(4, 0, FP8), e(4, 0), e(8, 0, FP8), e(1, 0), out)
+    assert bool((out == 0).all())
+    with pytest.raises(ops().KernelError, match="K is 0"):
+        ops().linear_fp8_swiglu(e(4, 0, FP8), e(4, 0), e(8, 0, FP8), e(1, 0), e(8, 0, FP8), e(1, 0), e(4, 8, FP8), e(4, 1))
+    ops().quantize_fp8(e(0, 256), e(0, 256, FP8), e(0, 2))
+    ops().add_gated_norms(e(0, 256), None, e(0, 256), weight=torch.ones(256, device=DEV))
+    torch.cuda.synchronize()
+
+
+def test_a_row_wider_than_a_block_holds_is_refused():
+    H = ops().GATED_NORMS_WIDTH + 8
+    x = torch.ones((2, H), device=DEV)
+    with pytest.raises(ops().KernelError, match="outside what this kernel takes"):
+        ops().add_gated_norms(x, None, torch.empty_like(x), weight=torch.ones(H, device=DEV))
+
+
+@pytest.mark.parametrize("T,K", [(1, 100_000), (20, 70_000), (32, 400_000)])
+def test_products_of_long_rows(T, K):
+    """Rows whose scales would not fit a tile's shared memory take a plan that holds none."""
+    check_product(T, 130, K, F32, T)
+    check_gated(T, 130, K, T, gate_factor=0.005)
+
+
+def test_matrices_of_more_than_2_to_the_31():
+    """More than 2^31 elements in a matrix: its last rows are right."""
+    T, N, K = 65_700, 32_800, 128
+    x, xs = quantized(300, K, 1, 1)
+    big_x, big_xs = ops().fp8_rows(T, K, DEV)
+    big_x.view(torch.uint8)[:] = 0
+    big_xs.fill_(1.0)
+    big_x.view(torch.uint8)[-300:] = x.view(torch.uint8)
+    big_xs[-300:] = xs
+    w, ws = quantized(N, K, 2, 128, 0.02)
+    out = torch.empty((T, N), device=DEV, dtype=BF)
+    ops().linear_fp8(big_x, big_xs, w, ws, out)
+    want, error = pf.product(x, xs, w, ws)
+    alone = out[-300:].clone()
+    assert bool(((alone.cpu().double() - want).abs() <= error + pf.half_step(want.abs() + error, BF)).all())
+    assert not bool(out[:1000].any())
+    q, s = ops().fp8_rows(T, N, DEV)
+    ops().quantize_fp8(out, q, s)
+    q1, s1 = ops().fp8_rows(300, N, DEV)
+    ops().quantize_fp8(alone, q1, s1)
+    assert torch.equal(q[-300:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s[-300:], s1)
+    blocks = torch.empty((groups(T), groups(N)), device=DEV)
+    ops().quantize_fp8(out, q, blocks, 128)
+    tail = T // 128 * 128
+    q1, s1 = ops().fp8_rows(T - tail, N, DEV)
+    last = torch.empty((1, groups(N)), device=DEV)
+    ops().quantize_fp8(out[tail:], q1, last, 128)
+    assert torch.equal(q[tail:].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(blocks[-1:], last)
+    del out, q, q1
+    rows = 140_000
+    stream = torch.zeros((rows, 16384), device=DEV, dtype=BF)
+    stream[-3:] = activations(3, 16384, 3, BF).to(DEV)
+    weight = torch.ones(16384, device=DEV)
+    q, s = ops().fp8_rows(rows, 16384, DEV)
+    ops().add_gated_norms(stream, None, q, s, weight=weight, eps=1e-6)
+    want = stream[-3:].double()
+    want = (want / torch.sqrt(want.square().mean(1, keepdim=True) + 1e-6)).cpu()
+    off = (pf.values(q[-3:], s[-3:], 1) - want).abs()
+    assert bool((off <= pf.quantized_error(want, s[-3:], want.abs() * 50 * EPS32)).all())
+    assert not bool(q[:3].view(torch.uint8).any())

@@ -47,15 +47,17 @@ def checked(ops, counts):
         counts["quantize"] += 1
         return out
 
-    def linear(x, xs, w, ws, out, plan=None):
-        ops["linear_fp8"](x, xs, w, ws, out, plan)
+    def linear(x, xs, w, ws, out, static_weights=False):
+        ops["linear_fp8"](x, xs, w, ws, out, static_weights)
+        assert static_weights
         y, error = pf.product(x.cpu(), xs.cpu(), w.cpu(), ws.cpu())
         near((out.cpu().double() - y).abs(), error + pf.half_step(y.abs() + error, out.dtype), "product")
         counts["linear"] += 1
         return out
 
-    def gated(x, xs, g, gs, u, us, out, so, plan=None):
-        ops["linear_fp8_swiglu"](x, xs, g, gs, u, us, out, so, plan)
+    def gated(x, xs, g, gs, u, us, out, so, static_weights=False):
+        ops["linear_fp8_swiglu"](x, xs, g, gs, u, us, out, so, static_weights)
+        assert static_weights
         yg, eg = pf.product(x.cpu(), xs.cpu(), g.cpu(), gs.cpu())
         yu, eu = pf.product(x.cpu(), xs.cpu(), u.cpu(), us.cpu())
         h = yg * torch.sigmoid(yg) * yu
