@@ -33,6 +33,8 @@ __device__ __forceinline__ bool ft_elect() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(yes));
     return yes != 0;
 }
+// a number in 0 .. 2^16 - 1 for each tile, neighbours far apart whatever it is divided by (Fibonacci hashing)
+__device__ __forceinline__ unsigned int ft_spread(int tile) { return (unsigned int)tile * 0x9E3779B1u >> 16; }
 __device__ __forceinline__ int ft_warp() { return __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0); }
 template <bool PAIR>
 __device__ __forceinline__ void ft_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
@@ -95,6 +97,11 @@ __device__ __forceinline__ bool ft_warp_failed(uint32_t bar, uint32_t parity, vo
     return !ok;
 }
 
+__device__ __forceinline__ float4 ft_read4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -106,25 +113,31 @@ __device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
 // cluster's CTAs and their warps share them), a lane four neighbouring features.  GATED: the features are units' gates, then the same
 // units' ups; a token's 128 units are a group and the warp holds it.  HALVES 1: a CTA has them all (BN 256); 2: it has 64 of them (BN 128),
 // the CTAs of even rank the first 64, those of odd rank the others.
-// AT_ONCE: tokens that a warp fetches together (another CTA's shared memory is half a microsecond away under load).
-template <int BN, bool GATED, int HALVES, int AT_ONCE>
+// AT_ONCE: tokens that a warp takes together (another CTA's shared memory is half a microsecond away under load; of the gated form's
+// scales its lanes make one each, side by side).  ALONE: the CTA is its whole cluster.
+template <int BN, bool GATED, int HALVES, int AT_ONCE, bool ALONE>
 __device__ __forceinline__ void ft_emit(const Fp8TcParams& p, uint32_t at, int ld, int first, int step, int rows, int row0, int tb) {
     const int lane = threadIdx.x & 31, half = HALVES == 2 ? lane >> 4 : 0;
     // the sums of features c .. c + 3 and the tokens r, r + step, ..
     auto sum4 = [&](int r, int c, float4 (&v)[AT_ONCE]) {
-        float4 o[AT_ONCE][8];
+        if constexpr (ALONE) {
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j)
+            for (int j = 0; j < AT_ONCE; ++j) v[j] = ft_read4(at + (uint32_t)(min(r + j * step, rows - 1) * ld + c) * 4);
+        } else {
+            float4 o[AT_ONCE][8];
 #pragma unroll
-            for (int q = 0; q < 8 / HALVES; ++q)
-                if (q < p.splits)
-                    o[j][q] = ft_cluster_read4(cluster_map(at + (uint32_t)(min(r + j * step, rows - 1) * ld + c) * 4, q * HALVES + half));
+            for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; ++j) {
-            v[j] = o[j][0];
+                for (int q = 0; q < 8 / HALVES; ++q)
+                    if (q < p.splits)
+                        o[j][q] = ft_cluster_read4(cluster_map(at + (uint32_t)(min(r + j * step, rows - 1) * ld + c) * 4, q * HALVES + half));
 #pragma unroll
-            for (int q = 1; q < 8 / HALVES; ++q)
-                if (q < p.splits) { v[j].x += o[j][q].x; v[j].y += o[j][q].y; v[j].z += o[j][q].z; v[j].w += o[j][q].w; }
+            for (int j = 0; j < AT_ONCE; ++j) {
+                v[j] = o[j][0];
+#pragma unroll
+                for (int q = 1; q < 8 / HALVES; ++q)
+                    if (q < p.splits) { v[j].x += o[j][q].x; v[j].y += o[j][q].y; v[j].z += o[j][q].z; v[j].w += o[j][q].w; }
+            }
         }
     };
 #pragma unroll 1
@@ -134,17 +147,23 @@ __device__ __forceinline__ void ft_emit(const Fp8TcParams& p, uint32_t at, int l
             float4 gs[AT_ONCE], us[AT_ONCE];
             sum4(r, c, gs);
             sum4(r, BN / 2 + c, us);
+            uint32_t own = 0;
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j) {
+                float4 &h = gs[j], &u = us[j];
+                h.x = fp8_silu(h.x) * u.x; h.y = fp8_silu(h.y) * u.y; h.z = fp8_silu(h.z) * u.z; h.w = fp8_silu(h.w) * u.w;
+                uint32_t m = max(max(fp8_magnitude(h.x), fp8_magnitude(h.y)), max(fp8_magnitude(h.z), fp8_magnitude(h.w)));
+                m = __reduce_max_sync(0xffffffffu, m);
+                if (lane % AT_ONCE == j) own = m;
+            }
+            const Fp8Scale k = fp8_scale(own);              // of token lane % AT_ONCE
+#pragma unroll
+            for (int j = 0; j < AT_ONCE; ++j) {
+                const float by = __shfl_sync(0xffffffffu, k.r, j);
                 if (r + j * step >= rows) break;
                 const size_t row = (size_t)(row0 + r + j * step);
-                const float4 g = gs[j], u = us[j];
-                const float h[4] = {fp8_silu(g.x) * u.x, fp8_silu(g.y) * u.y, fp8_silu(g.z) * u.z, fp8_silu(g.w) * u.w};
-                uint32_t m = max(max(fp8_magnitude(h[0]), fp8_magnitude(h[1])), max(fp8_magnitude(h[2]), fp8_magnitude(h[3])));
-                m = __reduce_max_sync(0xffffffffu, m);
-                const Fp8Scale k = fp8_scale(m);
-                const uint32_t w = fp8_pack4(h[0], h[1], h[2], h[3], k.r);
-                if (lane == 0) p.so[row * p.ldso + tb] = k.s;
+                const uint32_t w = fp8_pack4(gs[j].x, gs[j].y, gs[j].z, gs[j].w, by);
+                if (lane == j) p.so[row * p.ldso + tb] = k.s;
                 const int u0 = tb * FT_ROWS + 4 * lane;
                 uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + row * p.ldo + u0;
                 if (p.out_vec && u0 + 4 <= p.N) {

@@ -43,7 +43,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     const int kb0 = split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.n_kb), t0 = ta * BT;
     // Each tile begins at another of its k-blocks and goes round: the CTAs, which start together, would all read the same tokens' bytes
     // at the same time (a tile's order is its own, whatever the others do).
-    const int count = kb1 - kb0, turned = (int)((unsigned)(tb * HALVES + half) * 5u % (unsigned)count);
+    const int count = kb1 - kb0, turned = (int)(ft_spread(tb * HALVES + half) % (unsigned)count);
     auto block_of = [&](int i) { return i + turned < count ? i + turned : i + turned - count; };
     if (threadIdx.x == 0) {
         abort_s = 0;
@@ -199,7 +199,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     }
     if (size > 1) cluster_sync_all();
     if (!abort_s)
-        ft_emit<FT_ROWS, GATED, HALVES, 1>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
+        ft_emit<FT_ROWS, GATED, HALVES, 1, false>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
     // (the peers may still read this CTA's sums)
     if (size > 1) cluster_sync_all();
 }

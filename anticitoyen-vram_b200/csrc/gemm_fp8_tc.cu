@@ -388,7 +388,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
 
     // Each column of tiles begins at another of its k-blocks (a multiple of four) and goes round: the CTAs, which start together, would
     // all read the same tokens' bytes at the same time (a tile's order is its own, whatever the others do).
-    const int count = kb1 - kb0, turned = (int)((unsigned)tb * 20u % (unsigned)count) & ~3, wrap = count - turned;
+    const int count = kb1 - kb0, turned = (int)(ft_spread(tb) % (unsigned)((count + 3) / 4)) * 4, wrap = count - turned;
     auto block_of = [&](int i) { return i < wrap ? i + turned : i - wrap; };
     if (warp == 0) {
         auto load_w = [&](int s, int kb) {
@@ -508,8 +508,11 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }
     if (p.splits > 1) cluster_sync_all();
-    if (!abort_s)
-        ft_emit<BN, GATED, 1, 2>(p, tiles_addr, S::LD, split + p.splits * warp, p.splits * (S::THREADS / 32), min(FT_ROWS, p.M - row_here), row_here, tb);
+    if (!abort_s) {
+        const int first = split + p.splits * warp, step = p.splits * (S::THREADS / 32), rows = min(FT_ROWS, p.M - row_here);
+        if (p.splits == 1) ft_emit<BN, GATED, 1, 4, true>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+        else ft_emit<BN, GATED, 1, 2, false>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+    }
     // (the peers may still read this CTA's sums)
     if (p.splits > 1) cluster_sync_all();
 }
