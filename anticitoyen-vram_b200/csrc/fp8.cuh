@@ -135,9 +135,10 @@ __device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {
     for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     return m;
 }
-// g sigmoid(g) in front of a rounding to e4m3 whose scale it decides: the exponential as CUDA gives it (two units), the quotient by the
-// hardware's approximation (two more; beyond 2^126 in the denominator it is 0, where the value is under 1e-36)
-__device__ __forceinline__ float fp8_silu(float g) { return __fdividef(g, 1.f + expf(-g)); }
+// g sigmoid(g) in front of a rounding to e4m3 whose scale it decides, a million times coarser than this: exponential and quotient by the
+// hardware's approximations (2 + 1.2 |g| units and two: where the exponential counts, for g under 0, the value is off by less than 2e-7;
+// beyond 2^126 in the denominator the quotient is 0, where the value is under 1e-36)
+__device__ __forceinline__ float fp8_silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
 static inline bool fp8_rows_aligned(const void* p, long long ld, int bytes, int to) {
     return !((uintptr_t)p % to) && !(ld * bytes % to);
 }

@@ -114,28 +114,28 @@ __device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
 // units' ups; a token's 128 units are a group and the warp holds it.  HALVES 1: a CTA has them all (BN 256); 2: it has 64 of them (BN 128),
 // the CTAs of even rank the first 64, those of odd rank the others.
 // AT_ONCE: tokens that a warp takes together (another CTA's shared memory is half a microsecond away under load; of the gated form's
-// scales its lanes make one each, side by side).  ALONE: the CTA is its whole cluster.
-template <int BN, bool GATED, int HALVES, int AT_ONCE, bool ALONE>
+// scales its lanes make one each, side by side).  SPLITS: the most shares a sum may have here; 1: the CTA is its whole cluster.
+template <int BN, bool GATED, int HALVES, int AT_ONCE, int SPLITS>
 __device__ __forceinline__ void ft_emit(const Fp8TcParams& p, uint32_t at, int ld, int first, int step, int rows, int row0, int tb) {
     const int lane = threadIdx.x & 31, half = HALVES == 2 ? lane >> 4 : 0;
     // the sums of features c .. c + 3 and the tokens r, r + step, ..
     auto sum4 = [&](int r, int c, float4 (&v)[AT_ONCE]) {
-        if constexpr (ALONE) {
+        if constexpr (SPLITS == 1 && HALVES == 1) {
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j) v[j] = ft_read4(at + (uint32_t)(min(r + j * step, rows - 1) * ld + c) * 4);
         } else {
-            float4 o[AT_ONCE][8];
+            float4 o[AT_ONCE][SPLITS];
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j)
 #pragma unroll
-                for (int q = 0; q < 8 / HALVES; ++q)
+                for (int q = 0; q < SPLITS; ++q)
                     if (q < p.splits)
                         o[j][q] = ft_cluster_read4(cluster_map(at + (uint32_t)(min(r + j * step, rows - 1) * ld + c) * 4, q * HALVES + half));
 #pragma unroll
             for (int j = 0; j < AT_ONCE; ++j) {
                 v[j] = o[j][0];
 #pragma unroll
-                for (int q = 1; q < 8 / HALVES; ++q)
+                for (int q = 1; q < SPLITS; ++q)
                     if (q < p.splits) { v[j].x += o[j][q].x; v[j].y += o[j][q].y; v[j].z += o[j][q].z; v[j].w += o[j][q].w; }
             }
         }

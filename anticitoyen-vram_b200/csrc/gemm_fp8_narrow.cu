@@ -199,7 +199,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     }
     if (size > 1) cluster_sync_all();
     if (!abort_s)
-        ft_emit<FT_ROWS, GATED, HALVES, 1, false>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
+        ft_emit<FT_ROWS, GATED, HALVES, 1, 8 / HALVES>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
     // (the peers may still read this CTA's sums)
     if (size > 1) cluster_sync_all();
 }

@@ -510,8 +510,9 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     if (p.splits > 1) cluster_sync_all();
     if (!abort_s) {
         const int first = split + p.splits * warp, step = p.splits * (S::THREADS / 32), rows = min(FT_ROWS, p.M - row_here);
-        if (p.splits == 1) ft_emit<BN, GATED, 1, 4, true>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
-        else ft_emit<BN, GATED, 1, 2, false>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+        if (p.splits == 1) ft_emit<BN, GATED, 1, 4, 1>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+        else if (p.splits <= 4) ft_emit<BN, GATED, 1, 4, 4>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+        else ft_emit<BN, GATED, 1, 2, 8>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
     }
     // (the peers may still read this CTA's sums)
     if (p.splits > 1) cluster_sync_all();
