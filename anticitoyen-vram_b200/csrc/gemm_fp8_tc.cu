@@ -8,8 +8,8 @@
 // sums that they hold in registers (a fused multiply-add for each output and k-block, two at a time as fma.rn.f32x2).  Tokens are
 // the rows (a lane holds one, so sx is a number of the thread's), features the columns, 64 or 128 of them to a thread.
 //
-// Two forms.  Pairs of CTAs on tiles of 256 x 256 (cta_group::2), persistent, for many tokens: a CTA loads 128 rows of each operand
-// for a k-block, 32 KB for 512 cycles of tensor core.  And single CTAs on tiles of 128 x BN, one each, for fewer: K may be split over
+// Two forms.  Pairs of CTAs on tiles of 256 x 256 or somewhat less (cta_group::2), persistent, for many tokens: a CTA loads 128 rows of each
+// operand for a k-block, 32 KB for 512 cycles of tensor core.  And single CTAs on tiles of 128 x BN, one each, for fewer: K may be split over
 // the CTAs of a cluster, whose sums meet through its shared memory, in rank order, so the result does not depend on timing.
 //
 // What bounds the many-token form beside the tensor core is that hand-over, once for each k-block: from the products' end until the
@@ -24,9 +24,9 @@
 #include "fp8_tc.cuh"
 
 // sums[0 .. 8 PIECES) += scales * 16 PIECES columns of this lane's row, the first half of them from `first`, the others from `second`;
-// a piece of sixteen is on its way while the one before is added
+// a piece of sixteen is on its way while the one before is added.  Pieces from `change` on have the second scale.
 template <int PIECES>
-__device__ __forceinline__ void ft_add_tile(uint64_t* sums, uint32_t first, uint32_t second, float scale1, float scale2) {
+__device__ __forceinline__ void ft_add_tile(uint64_t* sums, uint32_t first, uint32_t second, float scale1, float scale2, int change = PIECES / 2) {
     const uint64_t s1 = ft_both(scale1), s2 = ft_both(scale2);
     uint32_t r[2][16];
     tc_ld16_nowait(first, r[0]);
@@ -35,7 +35,7 @@ __device__ __forceinline__ void ft_add_tile(uint64_t* sums, uint32_t first, uint
     for (int i = 0; i < PIECES; ++i) {
         if (i + 1 < PIECES) tc_ld16_nowait(i + 1 < PIECES / 2 ? first + 16 * (i + 1) : second + 16 * (i + 1 - PIECES / 2), r[(i + 1) & 1]);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) ft_fma2(sums[8 * i + c], r[i & 1][2 * c], r[i & 1][2 * c + 1], i < PIECES / 2 ? s1 : s2);
+        for (int c = 0; c < 8; ++c) ft_fma2(sums[8 * i + c], r[i & 1][2 * c], r[i & 1][2 * c + 1], i < change ? s1 : s2);
         if (i + 1 < PIECES) ft_wait_ld(r[(i + 1) & 1]);
     }
 }
@@ -120,19 +120,22 @@ __device__ __forceinline__ void ft_tile_of(int tile, int tiles_m, int tiles_n, i
     tb = r / rows;
     ta = g * group + (r - tb * rows);
 }
-// ----------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256
-#define FP_STAGE (2 * FT_TILE)              // a CTA's share of a k-block: 128 rows of tokens, 128 of weights
+// ----------------------------------------------------------------------------- pairs of CTAs, tiles of 256 x 256 and less
+#define FP_STAGE (2 * FT_TILE)              // a CTA's share of a k-block: 128 rows of tokens, 128 of weights or less
 #define FP_MAX_STAGES 6
 #define FP_THREADS 320
 #define FP_SLOTS 2                          // partial tiles in tensor memory
 
+// PIECES: a tile is 256 x 32 PIECES, an epilogue thread has 16 PIECES of its columns; where that is not 128, the thread's columns may lie in
+// two blocks of the weights' scales.
 // GATED: the tile's columns are 128 units' gate rows (the leader's half of the weight tile) and the same units' up rows (the other's).
-template <bool GATED>
+template <bool GATED, int PIECES>
 __global__ void __launch_bounds__(FP_THREADS, 1)
 gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_w2, const Fp8TcParams p) {
     extern __shared__ unsigned char smem_raw[];
     unsigned char* tiles = smem_raw + ((1024u - (gt_smem(smem_raw) & 1023u)) & 1023u);
+    constexpr int COLS = 16 * PIECES, BYTES = 2 * (FT_TILE + COLS * FT_ROWS);       // of a thread or of a CTA's weight rows; of both CTAs' k-block
     const int STAGES = p.stages;
     const uint32_t tiles_addr = gt_smem(tiles);
     // barriers: full[STAGES] (the leader's count both CTAs' bytes), empty[STAGES], tmem_full[SLOTS], tmem_empty[SLOTS] (the leader's)
@@ -168,7 +171,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const CUtensorMap* weights = GATED && rank == 1 ? &map_w2 : &map_w;
         auto load_w = [&](int s, int kb, int tb) {
             tma_load_2d_pair(tiles_addr + s * FP_STAGE + FT_TILE, weights, lead_full0 + 8 * s, kb * FT_ROWS,
-                             GATED ? tb * FT_ROWS : tb * 2 * FT_ROWS + (int)rank * FT_ROWS);
+                             GATED ? tb * FT_ROWS : (tb * 2 + (int)rank) * COLS);
         };
         int early = 0, asked = 0;
         if (p.early_w && pair < n_items) {
@@ -177,7 +180,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             early = min(STAGES, p.n_kb);
             if (ft_elect()) {
                 for (int i = 0; i < early; ++i) {
-                    if (rank == 0) mbar_expect_tx(full0 + 8 * i, 2 * FP_STAGE);
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * i, BYTES);
                     load_w(i, i, tb);
                 }
             }
@@ -199,7 +202,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                     if (failed) break;
                 }
                 if (ft_elect()) {
-                    if (!half_done && rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * FP_STAGE);
+                    if (!half_done && rank == 0) mbar_expect_tx(full0 + 8 * s, BYTES);
                     if (kb != p.skip_kb) {
                         tma_load_2d_pair(tiles_addr + s * FP_STAGE, &map_x, lead_full0 + 8 * s, kb * FT_ROWS, row);
                         if (!half_done) load_w(s, kb, tb);
@@ -215,7 +218,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     } else if (warp == 1) {
         if (rank == 0) {
             pdl_wait();         // (the first tokens come after it: the wait for them starts there)
-            const uint32_t idesc = ft_idesc(2 * FT_ROWS, 2 * FT_ROWS);
+            const uint32_t idesc = ft_idesc(2 * COLS, 2 * FT_ROWS);
             const uint64_t a0 = umma_desc(tiles_addr), b0 = umma_desc(tiles_addr + FT_TILE);
             uint32_t turn = 0, ph = 0;
             int s = 0;
@@ -244,7 +247,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         const int wq = warp & 3, part = (warp - 2) >> 2;
         pdl_wait();
         const uint32_t lead_tempty0 = cluster_map(tempty0, 0);
-        const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16) + part * (GATED ? 64 : FT_ROWS);
+        const uint32_t taddr = tmem_base + ((uint32_t)(wq * 32) << 16) + part * (GATED ? 64 : COLS);
         uint32_t turn = 0, parity = 0;
         // (a warp gives up as a whole: its loads from tensor memory and its exchanges are the whole warp's)
         bool failed = false;
@@ -254,26 +257,30 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             const int row = ta * 2 * FT_ROWS + (int)rank * FT_ROWS + wq * 32 + lane;
             // (rows and blocks that do not exist have products of zeros: any scale that does exist will do)
             const float* sx = p.sx + (size_t)min(row, p.M - 1) * p.ldsx;
-            const int block = GATED ? tb : min(tb * 2 + part, (p.N - 1) / FT_ROWS);
-            const float *sw = p.sw + (size_t)block * p.ldsw, *sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : nullptr;
-            uint64_t sums[64];
+            constexpr bool TWO = GATED || PIECES < 8;
+            const int column = (tb * 2 + part) * COLS, last_block = (p.N - 1) / FT_ROWS, block = GATED ? tb : min(column / FT_ROWS, last_block);
+            const int change = GATED || PIECES == 8 ? PIECES / 2 : (FT_ROWS - column % FT_ROWS) / 16;       // (the first piece of the next block)
+            const float* sw = p.sw + (size_t)block * p.ldsw;
+            const float* sw2 = GATED ? p.sw2 + (size_t)block * p.ldsw2 : p.sw + (size_t)min(block + 1, last_block) * p.ldsw;
+            uint64_t sums[8 * PIECES];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) sums[i] = 0;
+            for (int i = 0; i < 8 * PIECES; ++i) sums[i] = 0;
             FtRowScales xs;
             xs.begin(sx, p.n_kb, p.sx_vec);
-            float next_w = sw[0], next_w2 = GATED ? sw2[0] : 0.f;
+            float next_w = sw[0], next_w2 = TWO ? sw2[0] : 0.f;
             for (int kb = 0; kb < p.n_kb; ++kb, ++turn) {
-                const float x = xs.take(kb), s1 = x * next_w, s2 = GATED ? x * next_w2 : s1;
+                const float x = xs.take(kb), s1 = x * next_w, s2 = TWO ? x * next_w2 : s1;
                 if (kb + 1 < p.n_kb) {
                     next_w = sw[kb + 1];
-                    if (GATED) next_w2 = sw2[kb + 1];
+                    if (TWO) next_w2 = sw2[kb + 1];
                 }
                 const uint32_t slot = turn % FP_SLOTS, use = turn / FP_SLOTS;
                 failed = ft_warp_failed(tfull0 + 8 * slot, use & 1, &abort_s, p);
                 if (failed) break;
                 tc_fence_after();
                 const uint32_t t = taddr + slot * 2 * FT_ROWS;
-                ft_add_tile<8>(sums, t, t + (GATED ? FT_ROWS : 64), s1, s2);
+                if (PIECES == 8) ft_add_tile<8>(sums, t, t + (GATED ? FT_ROWS : 64), s1, s2);
+                else ft_add_tile<PIECES>(sums, t, t + PIECES / 2 * 16, s1, s2, change);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -284,8 +291,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             if (failed) break;
             if (!GATED) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    ft_store16(p, row, tb * 2 * FT_ROWS + part * FT_ROWS + 16 * i, sums + 8 * i);
+                for (int i = 0; i < PIECES; ++i) ft_store16(p, row, column + 16 * i, sums + 8 * i);
             } else {
                 // silu(gate) * up of 64 units, in the place of the gates' sums; the other 64 of the group are the partner warp's
                 uint32_t m = 0;
@@ -529,11 +535,11 @@ ACV_API void acv_gemm_fp8_test_fault(int wait_limit, int skip_kb) {
     g_test_skip_kb = skip_kb;
 }
 
-template <bool GATED>
+template <bool GATED, int PIECES>
 static int ft_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mw2, Fp8TcParams& p, int sms, cudaStream_t stream) {
     p.stages = FP_MAX_STAGES;
     const int smem = FP_MAX_STAGES * FP_STAGE + 1024 + 256;
-    auto kernel = gemm_fp8_pair_kernel<GATED>;
+    auto kernel = gemm_fp8_pair_kernel<GATED, PIECES>;
     static AcvSmemConfig cfg;
     if (const int rc = acv_ensure_smem(cfg, kernel, smem)) return rc;
     // pairs that can be resident at once: two free SMs side by side each, which an odd number of SMs in a part of the chip does not give
@@ -562,7 +568,8 @@ static int ft_launch_pair(const CUtensorMap& mx, const CUtensorMap& mw, const CU
         }
     }
     p.tiles_m = (p.M + 2 * FT_ROWS - 1) / (2 * FT_ROWS);
-    p.tiles_n = (p.N + (GATED ? 1 : 2) * FT_ROWS - 1) / ((GATED ? 1 : 2) * FT_ROWS);
+    const int wide = GATED ? FT_ROWS : 32 * PIECES;
+    p.tiles_n = (p.N + wide - 1) / wide;
     p.group = 8;
     const long long items = (long long)p.tiles_m * p.tiles_n;
     if (items > 0x7fffffff) return ACV_ERR_SIZE;
@@ -592,7 +599,7 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
     return acv_launch_status();
 }
 
-// How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs, 4 weight
+// How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs on tiles of 256 x bn, 4 weight
 // rows on the tensor core's rows, bn tokens to a tile, K over `splits` CTAs (gemm_fp8_narrow.cu).
 //
 // Up to 16 tokens whose weights are one round of blocks of 32 rows stream (microseconds, streaming and the best of kind 4: 8 tokens
@@ -604,9 +611,11 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
 // in 1, 2, 4: 4.3, 3.8, 4.2; 12288 units, K 4096, in 1, 2, 3: 21.0, 19.2, 24.8; kind 2, 65 tokens 4096 x 12288 in 2, 3, 4, 6: 19.5, 15.9,
 // 14.0, 23.3.  Kind 4 holds the scales of its k-blocks in shared memory beside its stages: 160 KB of them at most, about 80 thousand k to a
 // split of 32 tokens' gated form, and longer rows are kind 2's (one that holds none).
-//   Pairs of CTAs and tiles of 128 rows both come in rounds over the SMs, and a round of pairs takes 1.3 of a round of tiles of 128 x 128,
-// 0.83 of one of gated tiles of 128 x 256 (K 4096: 16.2 us, 21; 37.5, 31.2): 512 tokens 4096 x 4096 16.2 and 19.8, 6144 x 4096 32.1 and 22.5,
-// 384 tokens of 12288 units 76 and 93, 512 of them 113 and 94.
+//   Pairs of CTAs and tiles of 128 rows both come in rounds over the SMs.  A round of pairs takes 1.5 of a round of tiles of 128 x 128
+// (1024 tokens 5120 x 17408 in 2 and 3: 143 us and 136; 6144 x 4096, 512 tokens in 1 and 2: 28, 32; 2048 in 3 and 6: 63, 82), 0.83 of
+// one of gated tiles of 128 x 256 (12288 units of 4096, 256 tokens in 2 and 2: 43.8, 50.1; 384 in 3 and 2: 69, 54).  Pairs take tiles of
+// 256 columns, or of 224 or 192 where those come in few enough rounds: such a round takes 0.94 and 0.87 (with 256, 224 and 192 columns, 1024
+// tokens 7168 x 5120 in 2, 2, 3 rounds 49.7, 46.1, 57.4; 5120 x 17408 in 2, 2, 2: 143, 135, 122; 4096 tokens 4096 x 12288 in 4, 5, 5: 202, 257, 234).
 struct Fp8Plan { int kind, bn, splits; };
 static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
     const long long n_kb = (K + FT_ROWS - 1) / FT_ROWS, wide = (N + FT_ROWS - 1) / FT_ROWS, deep = (M + FT_ROWS - 1) / FT_ROWS;
@@ -621,9 +630,15 @@ static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
         if ((n_kb + splits - 1) / splits * (gated ? 2 : 1) * (bt + 1) * 4 <= 160 * 1024) return {4, bt, splits};
         splits = 1;
     }
-    const long long tiles = deep * wide, pairs = (deep + 1) / 2 * (gated ? wide : (wide + 1) / 2);
-    const long long tile_rounds = (tiles + sms - 1) / sms, pair_rounds = (pairs + sms / 2 - 1) / (sms / 2);
-    if ((double)pair_rounds * (gated ? 0.83 : 1.3) < (double)tile_rounds) return {3, 256, 1};
+    const long long tiles = deep * wide, tile_rounds = (tiles + sms - 1) / sms;
+    auto rounds_of = [&](long long across) { return (double)(((deep + 1) / 2 * across + sms / 2 - 1) / (sms / 2)); };
+    if (gated) {
+        if (rounds_of(wide) * 0.83 < (double)tile_rounds) return {3, 256, 1};
+    } else {
+        const double by256 = rounds_of((wide + 1) / 2), by224 = rounds_of((N + 223) / 224) * 0.94, by192 = rounds_of((N + 191) / 192) * 0.87;
+        const double least = min(by256, min(by224, by192));
+        if (least * 1.5 < (double)tile_rounds) return {3, by256 <= least ? 256 : by224 <= least ? 224 : 192, 1};
+    }
     while (splits < 8 && tiles <= fit(splits + 1) && n_kb >= 4 * (splits + 1)) ++splits;
     return {2, gated ? 256 : 128, splits};
 }
@@ -654,11 +669,17 @@ static int ft_run(Fp8Operands& o, int flags, int plan, int* status, int sms, cud
     if (how.kind == 4 && how.bn != 16 && how.bn != 32) return ACV_ERR_SIZE;
     if (how.kind == 2 && how.bn != (gated ? 256 : 128)) return ACV_ERR_SIZE;
     if (const int rc = ft_map(&mx, o.x, o.M, o.K, o.ldx, how.kind == 4 ? how.bn : FT_ROWS)) return rc;
-    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 4 && gated ? 64 : FT_ROWS)) return rc;
+    if (how.kind == 3 && how.bn != 256 && (gated || (how.bn != 224 && how.bn != 192))) return ACV_ERR_SIZE;
+    if (const int rc = ft_map(&mw, o.w, o.N, o.K, o.ldw, how.kind == 4 && gated ? 64 : how.kind == 3 ? how.bn / 2 : FT_ROWS)) return rc;
     mw2 = mw;
     if (gated)
         if (const int rc = ft_map(&mw2, o.w2, o.N, o.K, o.ldw2, how.kind == 4 ? 64 : FT_ROWS)) return rc;
-    if (how.kind == 3) return gated ? ft_launch_pair<true>(mx, mw, mw2, p, sms, stream) : ft_launch_pair<false>(mx, mw, mw2, p, sms, stream);
+    if (how.kind == 3) {
+        if (gated) return ft_launch_pair<true, 8>(mx, mw, mw2, p, sms, stream);
+        return how.bn == 256   ? ft_launch_pair<false, 8>(mx, mw, mw2, p, sms, stream)
+               : how.bn == 224 ? ft_launch_pair<false, 7>(mx, mw, mw2, p, sms, stream)
+                               : ft_launch_pair<false, 6>(mx, mw, mw2, p, sms, stream);
+    }
     if (how.kind == 4) return acv_fp8_narrow(mx, mw, mw2, p, gated, how.bn, how.splits, sms, stream);
     if (how.kind != 2) return ACV_ERR_SIZE;
     return gated ? ft_launch_tile<256, true>(mx, mw, mw2, p, how.splits, stream) : ft_launch_tile<128, false>(mx, mw, mw2, p, how.splits, stream);

@@ -134,7 +134,7 @@ def test_product_of_other_sizes(T, N, K):
     check_product(T, N, K, F32, T + N + K, (1, 2, 3))
 
 
-@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 128, 1), (2, 128, 2), (2, 128, 8), (3, 256, 1), (4, 16, 1), (4, 16, 8), (4, 32, 2)])
+@pytest.mark.parametrize("plan", [(1, 0, 1), (2, 128, 1), (2, 128, 2), (2, 128, 8), (3, 256, 1), (3, 224, 1), (3, 192, 1), (4, 16, 1), (4, 16, 8), (4, 32, 2)])
 @pytest.mark.parametrize("T,N,K,out_dtype", [(16, 257, 2048, F32), (1, 128, 128, F32), (5, 300, 400, BF), (140, 130, 1100, F32), (300, 700, 2048, BF), (513, 257, 1296, F32)])
 def test_product_by_every_plan(T, N, K, out_dtype, plan):
     if plan[0] == 1 and T > 16:
@@ -146,7 +146,8 @@ def test_product_by_every_plan(T, N, K, out_dtype, plan):
 
 def test_products_of_many_tiles():
     """More tiles than multiprocessors, so that a pair of CTAs walks several."""
-    check_product(1500, 6000, 272, BF, 5, plan=(3, 256, 1))
+    for columns in (256, 224, 192):
+        check_product(1500, 6000, 272, BF, 5, plan=(3, columns, 1))
     check_gated(1500, 4000, 272, 5, plan=(3, 256, 1))
 
 
