@@ -140,15 +140,22 @@ class Fp8Linear:
 
     @staticmethod
     def needs(name: str, out_features: int, in_features: int) -> dict[str, TensorNeed]:
-        """The tensors of the weight called ``name``."""
+        """The tensors of the weight called ``name`` (a bias beside it is known by name, and refused when the weight is loaded)."""
         blocks = tuple(-(-n // ops.FP8_GROUP) for n in (out_features, in_features))
         return {name: TensorNeed((out_features, in_features), "fp8"),
-                name + "_scale_inv": TensorNeed(blocks, "scale", optional=True)}
+                name + "_scale_inv": TensorNeed(blocks, "scale", optional=True),
+                Fp8Linear._bias_of(name): TensorNeed((out_features,), "bias", optional=True)}
+
+    @staticmethod
+    def _bias_of(name: str) -> str:
+        return name.removesuffix("weight") + "bias"
 
     @staticmethod
     def matrix(tensors, name: str, device) -> tuple[torch.Tensor, torch.Tensor]:
         """(values, scales) on the device of the weight called ``name``."""
         w, scales = tensors[name], tensors.get(name + "_scale_inv")
+        if tensors.get(Fp8Linear._bias_of(name)) is not None:
+            raise WeightError(name, unexpected=[Fp8Linear._bias_of(name) + " (8-bit weights are built without biases)"])
         if w.dtype == ops.FP8:
             if scales is None:
                 raise WeightError(name, missing=[name + "_scale_inv"])

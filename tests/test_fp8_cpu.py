@@ -173,3 +173,14 @@ def test_command_line_has_the_choice():
     args = build_parser().parse_args(["generate", "folder", "--weights", "fp8"])
     assert args.weights == "fp8"
     assert build_parser().parse_args(["bench", "folder"]).weights is None
+
+
+def test_a_bias_beside_8_bit_weights_is_refused():
+    """Weights in more bits are served with the biases that a file happens to hold; here they must not be left out in silence."""
+    from acvram_b200.parts.linear import Fp8Linear
+    from acvram_b200.weights.needs import WeightError
+    needs = Fp8Linear.needs("q_proj.weight", 256, 128)
+    assert needs["q_proj.bias"].optional and needs["q_proj.bias"].shape == (256,)
+    with pytest.raises(WeightError, match="q_proj.bias .*without biases"):
+        Fp8Linear.matrix({"q_proj.weight": torch.zeros((128, 128)).to(FP8), "q_proj.weight_scale_inv": torch.ones((1, 1)),
+                          "q_proj.bias": torch.ones(128)}, "q_proj.weight", "cpu")
