@@ -61,19 +61,25 @@ __device__ __forceinline__ void raw8_floats(const Raw8& r, int f32, float (&v)[8
         }
     }
 }
-// the same element by element, zeros from `n` on: for rows whose length, stride or start is not a multiple of 16 bytes
+// Rows whose length, stride or start is not a multiple of 16 bytes go element by element.  The sixteen lanes of a group of 128 then take
+// neighbouring elements, so that a load or store of a warp is two runs of sixteen: a lane's eight are 16 apart.
+template <bool VEC>
+__device__ __forceinline__ int piece_at(int piece) { return VEC ? piece * 8 : (piece & ~15) * 8 + (piece & 15); }
+template <bool VEC>
+__device__ __forceinline__ int piece_element(int at, int i) { return VEC ? at + i : at + 16 * i; }
+// eight elements of a row in that order, zeros from `n` on
 __device__ __forceinline__ void load8_ragged(const void* row, int f32, int at, int n, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        v[i] = at + i >= n ? 0.f : f32 ? reinterpret_cast<const float*>(row)[at + i] : __bfloat162float(reinterpret_cast<const bf16*>(row)[at + i]);
+        v[i] = at + 16 * i >= n ? 0.f : f32 ? reinterpret_cast<const float*>(row)[at + 16 * i] : __bfloat162float(reinterpret_cast<const bf16*>(row)[at + 16 * i]);
 }
 __device__ __forceinline__ Raw8 raw8_load_ragged(const void* row, int f32, int at, int n) {
     uint32_t w[8] = {};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (at + i < n) {
-            if (f32) w[i] = reinterpret_cast<const uint32_t*>(row)[at + i];
-            else w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[at + i] << (16 * (i & 1));
+        if (at + 16 * i < n) {
+            if (f32) w[i] = reinterpret_cast<const uint32_t*>(row)[at + 16 * i];
+            else w[i >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(row)[at + 16 * i] << (16 * (i & 1));
         }
     return {make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
 }
@@ -95,9 +101,9 @@ __device__ __forceinline__ void store8(void* row, int f32, int at, const float (
 __device__ __forceinline__ void store8_ragged(void* row, int f32, int at, int n, const float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (at + i < n) {
-            if (f32) reinterpret_cast<float*>(row)[at + i] = v[i];
-            else reinterpret_cast<bf16*>(row)[at + i] = __float2bfloat16_rn(v[i]);
+        if (at + 16 * i < n) {
+            if (f32) reinterpret_cast<float*>(row)[at + 16 * i] = v[i];
+            else reinterpret_cast<bf16*>(row)[at + 16 * i] = __float2bfloat16_rn(v[i]);
         }
 }
 template <bool VEC>
@@ -108,7 +114,7 @@ __device__ __forceinline__ void store_q8(uint8_t* row, int at, int n, const floa
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (at + i < n) row[at + i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+            if (at + 16 * i < n) row[at + 16 * i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
     }
 }
 __device__ __forceinline__ uint32_t magnitude8(const float (&v)[8]) {

@@ -47,7 +47,7 @@ __device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < C; ++i) {
-                const int at = (threadIdx.x + i * blockDim.x) * 8;
+                const int at = piece_at<VEC>(threadIdx.x + i * blockDim.x);
                 if (at < H) {
                     if (VEC) raw8_floats(dw[i], d_f32, d[i]);
                     else load8_ragged(dr, d_f32, at, H, d[i]);
@@ -60,7 +60,7 @@ __device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8
         }
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            const int at = piece_at<VEC>(threadIdx.x + i * blockDim.x);
             if (at >= H) continue;
             if (p.w1) {
                 if (C > 1) gn_load<VEC>(p.w1, 1, at, H, w1);
@@ -95,7 +95,7 @@ __device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8
     } else {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            const int at = piece_at<VEC>(threadIdx.x + i * blockDim.x);
             if (at >= H) continue;
             if (VEC) raw8_floats(xw[i], x_f32, x[i]);
             else load8_ragged(xr, x_f32, at, H, x[i]);
@@ -105,7 +105,7 @@ __device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < C; ++i)
-        if ((threadIdx.x + i * blockDim.x) * 8 < H) {
+        if (piece_at<VEC>(threadIdx.x + i * blockDim.x) < H) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) ss = fmaf(x[i][e], x[i][e], ss);
         }
@@ -115,11 +115,11 @@ __device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8
     uint32_t own = 0;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        const int at = (threadIdx.x + i * blockDim.x) * 8;
+        const int at = piece_at<VEC>(threadIdx.x + i * blockDim.x);
         const bool in = at < H;
         if (C > 1 && in) gn_load<VEC>(p.w2, 1, at, H, w2);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = (VEC ? in : at + e < H) ? x[i][e] * r * w2[e] : 0.f;      // (zeros behind the row's end)
+        for (int e = 0; e < 8; ++e) x[i][e] = (VEC ? in : piece_element<VEC>(at, e) < H) ? x[i][e] * r * w2[e] : 0.f;      // (zeros behind the row's end)
         if (p.out_kind == 2) {          // (whole warps pass here)
             const uint32_t m = half_warp_max(magnitude8(x[i]));
             if ((int)(threadIdx.x % C) == i) own = m;
@@ -133,7 +133,7 @@ __device__ __forceinline__ void gn_row(const GnParams& p, size_t row, const Raw8
     const Fp8Scale mine = fp8_scale(own);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        const int at = (threadIdx.x + i * blockDim.x) * 8;
+        const int at = piece_at<VEC>(threadIdx.x + i * blockDim.x);
         const float k = __shfl_sync(0xffffffffu, mine.r, i, 16);
         if (at < H) store_q8<VEC>(reinterpret_cast<uint8_t*>(o), at, H, x[i], k);
         const int group = (int)((threadIdx.x & ~15u) + i * blockDim.x) / 16;
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams
     if (VEC) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            const int at = (threadIdx.x + i * blockDim.x) * 8;
+            const int at = piece_at<VEC>(threadIdx.x + i * blockDim.x);
             if (at < H) {
                 const int x_f32 = gn_f32<XT>(p.x_f32), d_f32 = gn_f32<DT>(p.d_f32);
                 if (p.d) dw[i] = raw8_load(reinterpret_cast<const char*>(p.d) + row * p.ldd * (d_f32 ? 4 : 2), d_f32, at);
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams
     }
     float w1[8], w2[8], gc[8];
     if (C == 1) {
-        const int at = threadIdx.x * 8;
+        const int at = piece_at<VEC>(threadIdx.x);
         if (at < H) {
             if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
             if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);

@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const void* __res
             row += step_rows;
             g += step_groups;
             if (g >= G) { g -= G; ++row; }
-            const int at = gs[u] * FP8_GROUP + lane * 8;
+            const int at = piece_at<VEC>(gs[u] * 16 + lane);
             const char* src = reinterpret_cast<const char*>(x) + (size_t)rows[u] * ldx * esz;
             raw[u].a = raw[u].b = make_uint4(0, 0, 0, 0);
             if (rows[u] < T && at < K) {
@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(256, 4) quantize_rows_kernel(const void* __res
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const float r = __shfl_sync(0xffffffffu, mine.r, u, 16);
-            const int at = gs[u] * FP8_GROUP + lane * 8;
+            const int at = piece_at<VEC>(gs[u] * 16 + lane);
             if (rows[u] < T) {
                 if (at < K) {
                     raw8_floats(raw[u], f32, v);
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __rest
     __shared__ uint32_t red[8];
     pdl_launch_dependents();
     pdl_wait();
-    const int at = blockIdx.x * FP8_GROUP + (threadIdx.x & 15) * 8;
+    const int at = piece_at<VEC>(blockIdx.x * 16 + (threadIdx.x & 15));
     const int row0 = blockIdx.y * FP8_GROUP + (threadIdx.x >> 4), f32 = TYPE == 2 ? said : TYPE;
     const size_t esz = f32 ? 4 : 2;
     Raw8 raw[8];
