@@ -18,6 +18,7 @@ struct GnParams {
     float* s;
     long long ldx, ldd, ldg, ldo, lds;
     int H, x_f32, d_f32, g_f32, out_kind;       // out_kind: 0 float, 1 bfloat16, 2 e4m3, 3 none
+    int early_w;                                // the weights may be read before the kernel in front has ended
     float c, e1, e2, inv_h;
 };
 
@@ -147,6 +148,15 @@ __global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams
     __shared__ float red[32];
     pdl_launch_dependents();
     const int H = p.H;
+    float w1[8], w2[8], gc[8];
+    auto weights = [&]() {
+        const int at = piece_at<VEC>(threadIdx.x);
+        if (C > 1 || at >= H) return;
+        if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
+        if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
+        if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
+    };
+    if (p.early_w) weights();
     pdl_wait();
     const size_t row = blockIdx.x;
     Raw8 xw[C], dw[C], gw[C];
@@ -162,15 +172,7 @@ __global__ void __launch_bounds__(512, BLOCKS) gated_norms_kernel(const GnParams
             }
         }
     }
-    float w1[8], w2[8], gc[8];
-    if (C == 1) {
-        const int at = piece_at<VEC>(threadIdx.x);
-        if (at < H) {
-            if (p.w1) gn_load<VEC>(p.w1, 1, at, H, w1);
-            if (p.w2) gn_load<VEC>(p.w2, 1, at, H, w2);
-            if (p.gc) gn_load<VEC>(p.gc, 1, at, H, gc);
-        }
-    }
+    if (!p.early_w) weights();
     gn_row<VEC, C, XT, DT>(p, row, xw, dw, gw, w1, w2, gc, red);
 }
 
@@ -198,8 +200,8 @@ static int gn_launch(const GnParams& p, int T, int sms, cudaStream_t stream) {
 struct GatedNormsArgs {
     const void *x, *d, *g, *gc, *w1, *w2, *out, *s, *stream;
     long long ldx, ldd, ldg, ldo, lds;
-    int x_dtype, d_dtype, g_dtype, out_kind, T, H, sms;
-    float c, e1, e2, inv_h;
+    int x_dtype, d_dtype, g_dtype, out_kind, T, H, sms, early_w;
+    float c, e1, e2;
 };
 ACV_API int acv_add_gated_norms(const GatedNormsArgs* a) {
     const int T = a->T, H = a->H;
@@ -211,7 +213,7 @@ ACV_API int acv_add_gated_norms(const GatedNormsArgs* a) {
     p.w1 = a->d ? (const float*)a->w1 : nullptr; p.w2 = a->out_kind < 3 ? (const float*)a->w2 : nullptr;
     p.out = const_cast<void*>(a->out); p.s = (float*)const_cast<void*>(a->s);
     p.ldx = a->ldx; p.ldd = a->ldd; p.ldg = a->ldg; p.ldo = a->ldo; p.lds = a->lds; p.H = H;
-    p.x_f32 = a->x_dtype == ACV_F32; p.d_f32 = a->d_dtype == ACV_F32; p.g_f32 = a->g_dtype == ACV_F32; p.out_kind = a->out_kind;
+    p.x_f32 = a->x_dtype == ACV_F32; p.d_f32 = a->d_dtype == ACV_F32; p.g_f32 = a->g_dtype == ACV_F32; p.out_kind = a->out_kind; p.early_w = a->early_w;
     p.c = a->c; p.e1 = a->e1; p.e2 = a->e2; p.inv_h = 1.f / (float)H;
     const int ob = p.out_kind == 0 ? 4 : p.out_kind == 1 ? 2 : 1;
     const bool vec = H % 8 == 0 && fp8_rows_aligned(p.x, p.ldx, p.x_f32 ? 4 : 2, 16) && (!p.d || fp8_rows_aligned(p.d, p.ldd, p.d_f32 ? 4 : 2, 16)) &&

@@ -517,7 +517,8 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     if (!abort_s) {
         const int first = split + p.splits * warp, step = p.splits * (S::THREADS / 32), rows = min(FT_ROWS, p.M - row_here);
         if (p.splits == 1) ft_emit<BN, GATED, 1, 4, 1>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
-        else if (p.splits <= 4) ft_emit<BN, GATED, 1, 4, 4>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+        else if (p.splits <= 4 && rows > 2 * step) ft_emit<BN, GATED, 1, 4, 4>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
+        else if (rows <= step) ft_emit<BN, GATED, 1, 1, 8>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
         else ft_emit<BN, GATED, 1, 2, 8>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
     }
     // (the peers may still read this CTA's sums)
@@ -613,7 +614,8 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
 // split of 32 tokens' gated form, and longer rows are kind 2's (one that holds none).
 //   Pairs of CTAs and tiles of 128 rows both come in rounds over the SMs.  A round of pairs takes 1.5 of a round of tiles of 128 x 128
 // (1024 tokens 5120 x 17408 in 2 and 3: 143 us and 136; 6144 x 4096, 512 tokens in 1 and 2: 28, 32; 2048 in 3 and 6: 63, 82), 0.83 of
-// one of gated tiles of 128 x 256 (12288 units of 4096, 256 tokens in 2 and 2: 43.8, 50.1; 384 in 3 and 2: 69, 54).  Pairs take tiles of
+// one of gated tiles of 128 x 256 (12288 units of 4096, 256 tokens in 2 and 2: 43.8, 50.1; 384 in 3 and 2: 69, 54), and K over several CTAs brings a
+// round of those down with it (100 tokens of 8704 units of 5120, pairs and 2 splits: 31, 26; 39 of 1361 units of 11216, pairs and 8: 49, 16).  Pairs take tiles of
 // 256 columns, or of 224 or 192 where those come in few enough rounds: such a round takes 0.94 and 0.87 (with 256, 224 and 192 columns, 1024
 // tokens 7168 x 5120 in 2, 2, 3 rounds 49.7, 46.1, 57.4; 5120 x 17408 in 2, 2, 2: 143, 135, 122; 4096 tokens 4096 x 12288 in 4, 5, 5: 202, 257, 234).
 struct Fp8Plan { int kind, bn, splits; };
@@ -632,14 +634,14 @@ static Fp8Plan ft_plan(int M, int N, int K, bool gated, int sms) {
     }
     const long long tiles = deep * wide, tile_rounds = (tiles + sms - 1) / sms;
     auto rounds_of = [&](long long across) { return (double)(((deep + 1) / 2 * across + sms / 2 - 1) / (sms / 2)); };
+    while (splits < 8 && tiles <= fit(splits + 1) && n_kb >= 4 * (splits + 1)) ++splits;
     if (gated) {
-        if (rounds_of(wide) * 0.83 < (double)tile_rounds) return {3, 256, 1};
+        if (rounds_of(wide) * 0.83 < (splits > 1 ? 1. / splits + 0.25 : (double)tile_rounds)) return {3, 256, 1};
     } else {
         const double by256 = rounds_of((wide + 1) / 2), by224 = rounds_of((N + 223) / 224) * 0.94, by192 = rounds_of((N + 191) / 192) * 0.87;
         const double least = min(by256, min(by224, by192));
         if (least * 1.5 < (double)tile_rounds) return {3, by256 <= least ? 256 : by224 <= least ? 224 : 192, 1};
     }
-    while (splits < 8 && tiles <= fit(splits + 1) && n_kb >= 4 * (splits + 1)) ++splits;
     return {2, gated ? 256 : 128, splits};
 }
 

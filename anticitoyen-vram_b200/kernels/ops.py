@@ -2395,7 +2395,7 @@ def fp8_rows(rows: int, columns: int, device) -> tuple[torch.Tensor, torch.Tenso
 # and only a call that is refused, or has a column of a single element, goes through the words about it.
 _LINEAR_ARGS = struct.Struct("@10Q8q7i")        # Fp8LinearArgs
 _QUANTIZE_ARGS = struct.Struct("@4Q3q5i")       # QuantizeFp8Args
-_NORMS_ARGS = struct.Struct("@9Q5q7i3f")        # GatedNormsArgs
+_NORMS_ARGS = struct.Struct("@9Q5q8i3f")        # GatedNormsArgs
 _entries: dict = {}
 
 
@@ -2535,13 +2535,14 @@ _NORM_OUT = {torch.float32: 0, torch.bfloat16: 1, FP8: 2}
 
 def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tensor | None, out_scales: torch.Tensor | None = None, *,
                     post_weight: torch.Tensor | None = None, post_eps: float = 0.0, gate: torch.Tensor | None = None,
-                    residual_scale: float = 1.0, weight: torch.Tensor | None = None, eps: float = 0.0) -> torch.Tensor | None:
+                    residual_scale: float = 1.0, weight: torch.Tensor | None = None, eps: float = 0.0, static_weights: bool = False) -> torch.Tensor | None:
     """The stream x [T, H] += residual_scale * gate * n, in place, n = delta / sqrt(mean(delta^2) + post_eps) * post_weight (without
     ``post_weight``: n = delta); then, with ``out``, out = x / sqrt(mean(x^2) + eps) * weight of the stream as it is kept.
 
     x and delta float32 or bfloat16; ``gate`` float32 [H], or [T, H] float32 or bfloat16; weights float32 [H].  out float32 or
     bfloat16, rounded once, or float8_e4m3fn with ``out_scales``: quantised in groups of 128 as ``quantize_fp8`` does.  Matrices
-    have dense rows at any stride; H up to 16384.  Sums and both statistics are 32-bit."""
+    have dense rows at any stride; H up to 16384.  Sums and both statistics are 32-bit.  ``static_weights``: the weights and a gate of [H]
+    were written long before this call and may be read while the kernels before it are still running."""
     shape, device = x.shape, x.get_device()
     T, H = shape
     floats = (torch.float32, torch.bfloat16)
@@ -2600,5 +2601,6 @@ def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tens
         _one_device(name, x, delta, gate, post_weight, weight if out is not None else None, out, out_scales)
     if T and H:
         _launch_record(device, name, _NORMS_ARGS, 8, x.data_ptr(), d_at, g_at, gc_at, w1_at, w2_at, out_at, s_at, xs[0], d_ld, g_ld, out_ld,
-                       s_ld, _DT[x.dtype], d_type, g_type, kind, T, H, _sms_of(device), residual_scale, post_eps, eps)
+                       s_ld, _DT[x.dtype], d_type, g_type, kind, T, H, _sms_of(device), 1 if static_weights else 0, residual_scale, post_eps,
+                       eps)
     return out

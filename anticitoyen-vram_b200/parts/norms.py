@@ -68,7 +68,8 @@ class RMSNorm(Norm):
         """The same for a part whose first products are 8-bit ones: sum, norm and quantisation in one kernel; ``dtype``: the
         parts' element type.  The norm's output is not rounded in between."""
         rows = Fp8Rows(x.shape[0], x.shape[1], x.device, dtype)
-        ops.add_gated_norms(x, delta, rows.values, rows.scales, residual_scale=delta_scale, weight=self.weight, eps=self.eps)
+        ops.add_gated_norms(x, delta, rows.values, rows.scales, residual_scale=delta_scale, weight=self.weight, eps=self.eps,
+                            static_weights=True)
         return rows
 
 

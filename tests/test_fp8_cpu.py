@@ -89,7 +89,7 @@ def test_records_are_as_long_as_the_structs():
     """Pointers, then 64-bit strides, then 32-bit fields: no padding in front of any of them, so the packed length is their sum."""
     assert ops._LINEAR_ARGS.size == 10 * 8 + 8 * 8 + 7 * 4
     assert ops._QUANTIZE_ARGS.size == 4 * 8 + 3 * 8 + 5 * 4
-    assert ops._NORMS_ARGS.size == 9 * 8 + 5 * 8 + 7 * 4 + 3 * 4
+    assert ops._NORMS_ARGS.size == 9 * 8 + 5 * 8 + 8 * 4 + 3 * 4
 
 
 def test_plain_quantisation_is_near_what_it_stands_for():

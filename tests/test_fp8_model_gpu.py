@@ -66,9 +66,10 @@ def checked(ops, counts):
         counts["gated"] += 1
         return out, so
 
-    def norms(x, delta, out, scales=None, *, residual_scale=1.0, weight=None, eps=0.0):
+    def norms(x, delta, out, scales=None, *, residual_scale=1.0, weight=None, eps=0.0, static_weights=False):
+        assert static_weights
         before, d = x.cpu().double(), None if delta is None else delta.cpu().double()
-        ops["add_gated_norms"](x, delta, out, scales, residual_scale=residual_scale, weight=weight, eps=eps)
+        ops["add_gated_norms"](x, delta, out, scales, residual_scale=residual_scale, weight=weight, eps=eps, static_weights=static_weights)
         kept = x.cpu().double()
         want = before if d is None else before + residual_scale * d
         near((kept - want).abs(), want.abs() * 2 * EPS32 + pf.half_step(want * (1 + EPS32), x.dtype), "stream")
