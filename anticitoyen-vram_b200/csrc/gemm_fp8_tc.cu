@@ -14,7 +14,7 @@
 //
 // What bounds the many-token form beside the tensor core is that hand-over, once for each k-block: from the products' end until the
 // epilogue warps of both CTAs have fetched the partial tile (some 500 cycles, the bandwidth of tensor memory) and the issuing warp has
-// learnt it (as many), with two partial tiles for 512 cycles of tensor core each.  4096 x 4096 x 12288: 204 us; 155 us with nobody to wait for.
+// learnt it (as many), with two partial tiles for 512 cycles of tensor core each.  4096 x 4096 x 12288: 202 us; 143 us with nobody to wait for.
 // Finer partial tiles, more epilogue warps or registers taken from the idle warps did not shorten it (four tiles of 128 columns 238 us,
 // sixteen warps 310).
 //
