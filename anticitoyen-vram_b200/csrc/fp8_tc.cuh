@@ -70,13 +70,17 @@ __device__ __forceinline__ float2 ft_floats(uint64_t v) {
     return make_float2(__uint_as_float(lo), __uint_as_float(hi));
 }
 
-// After a wait that ran out: the loads that are still under way write into this CTA's shared memory, so their stages are waited for
-// (each by the parity of the last of `asked` k-blocks that went into it), with a limit.
-__device__ __forceinline__ void ft_drain(uint32_t full0, int stages, int asked, unsigned int limit) {
-    for (int s = 0; s < stages && s < asked; ++s) {
-        const int last = (asked - 1 - s) / stages;
-        for (unsigned int i = 0; i < limit; ++i)
-            if (mbar_try_wait(full0 + 8 * s, last & 1)) break;
+// After a wait that ran out, by one warp, when every role has left its loop (before that nobody knows whether another will give up): what
+// is still under way, loads that write into shared memory and products that read it, is waited for before the CTA's memory goes back,
+// each stage by the parity of the last of the `uses` k-blocks that went into it.  `bars`: the stages' "full" barriers, uses: the k-blocks
+// asked for; or the "empty" ones and the k-blocks whose products were issued.  The limit is this wait's own: a load is microseconds
+// away however few polls the others were given, and one that never comes is not waited for longer than some 20 milliseconds (5 us a poll).
+#define FT_DRAIN_LIMIT (1u << 12)
+__device__ __forceinline__ void ft_drain(uint32_t bars, int stages, int uses) {
+    for (int s = 0; s < stages && s < uses; ++s) {
+        const int last = (uses - 1 - s) / stages;
+        for (unsigned int i = 0; i < FT_DRAIN_LIMIT; ++i)
+            if (mbar_try_wait(bars + 8 * s, last & 1)) break;
     }
 }
 
@@ -101,6 +105,10 @@ __device__ __forceinline__ float4 ft_read4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
+}
+// a number into another CTA's shared memory (there when the cluster has met)
+__device__ __forceinline__ void ft_tell(uint32_t addr, int v) {
+    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ float4 ft_cluster_read4(uint32_t addr) {
     float4 v;

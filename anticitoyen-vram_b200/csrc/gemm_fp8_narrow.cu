@@ -36,6 +36,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     float* scales = reinterpret_cast<float*>(tiles + area + 256);           // [k-block][64 rows each of gate and up, or one for all][token]
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_s;
+    __shared__ int asked_s, issued_s;           // k-blocks whose loads and whose products are issued
     const int warp = ft_warp(), lane = threadIdx.x & 31;
     constexpr int HALVES = GATED ? 2 : 1;
     const int size = p.splits * HALVES, rank = blockIdx.x % size, split = rank / HALVES, half = rank % HALVES;
@@ -97,7 +98,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             if (++s == STAGES) { s = 0; ph ^= 1; }
             ready = __all_sync(0xffffffffu, ft_ready(empty0 + 8 * s, ph ^ 1));
         }
-        if (failed || abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
+        if (lane == 0) asked_s = asked;
     } else if (warp == 1) {
         pdl_wait();
         const uint32_t idesc = ft_idesc(BT, FT_ROWS);
@@ -105,7 +106,8 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         uint32_t ph = 0;
         int s = 0;
         bool ready = false;
-        for (int i = 0; i < count; ++i) {
+        int i = 0;
+        for (; i < count; ++i) {
             const uint32_t slot = (uint32_t)i % S::SLOTS, use = (uint32_t)i / S::SLOTS;
             if ((!ready && ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) ||
                 (use && ft_warp_failed(tempty0 + 8 * slot, (use & 1) ^ 1, &abort_s, p, 2)))
@@ -122,6 +124,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             if (++s == STAGES) { s = 0; ph ^= 1; }
             ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));
         }
+        if (lane == 0) issued_s = i;
     } else {
         const int wq = warp & 3, et = threadIdx.x - 64;
         {
@@ -194,6 +197,10 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
+        if (abort_s) {
+            ft_drain(full0, STAGES, asked_s);
+            ft_drain(empty0, STAGES, issued_s);
+        }
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }

@@ -126,6 +126,38 @@ __device__ __forceinline__ void ft_tile_of(int tile, int tiles_m, int tiles_n, i
 #define FP_THREADS 320
 #define FP_SLOTS 2                          // partial tiles in tensor memory
 
+// The end of a pair of which a CTA gave up (both know it), by a warp of each.  One that stopped sooner asks for as many k-blocks as the other
+// did (no more than the stages hold: a stage is asked for again only when both CTAs' loads of its last k-block have been used), so that the
+// leader's barriers, which count both CTAs' loads, and with them the wait for what is under way come to their end.  What these loads
+// bring is nobody's, so it is the matrices' first tile.
+// (Nothing of this may cost the epilogue's loop registers, hence the numbers in shared memory; with the loop of loads unrolled tiles of 192
+// columns spilled, 197 -> 231 us for 2048 tokens 5120 x 17408.)
+struct FpEnd {
+    uint32_t tiles;                     // where the stages are, the barriers behind them
+    int asked, issued, other_asked;     // k-blocks whose loads and whose products are issued; the loads of the pair's other CTA
+    int other_abort;
+};
+template <int COLS>
+__device__ __forceinline__ void fp_settle(const volatile FpEnd& end, int stages, const CUtensorMap* map_x, const CUtensorMap* map_w) {
+    const uint32_t tiles = end.tiles, full0 = tiles + stages * FP_STAGE;
+    const int asked = max(end.asked, end.other_asked);
+    const bool leads = cluster_ctarank() == 0;
+#pragma unroll 1
+    for (int i = end.asked; i < asked; ++i) {
+        const uint32_t s = (uint32_t)i % (uint32_t)stages, stage = tiles + s * FP_STAGE, bar = cluster_map(full0 + 8 * s, 0);
+        if (ft_elect()) {
+            if (leads) mbar_expect_tx(full0 + 8 * s, 2 * (FT_TILE + COLS * FT_ROWS));
+            tma_load_2d_pair(stage, map_x, bar, 0, 0);
+            tma_load_2d_pair(stage + FT_TILE, map_w, bar, 0, 0);
+        }
+        __syncwarp();
+    }
+    if (leads) {
+        ft_drain(full0, stages, asked);
+        ft_drain(full0 + 8 * stages, stages, end.issued);
+    }
+}
+
 // PIECES: a tile is 256 x 32 PIECES, an epilogue thread has 16 PIECES of its columns; where that is not 128, the thread's columns may lie in
 // two blocks of the weights' scales.
 // GATED: the tile's columns are 128 units' gate rows (the leader's half of the weight tile) and the same units' up rows (the other's).
@@ -143,6 +175,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const uint32_t tempty0 = tfull0 + 8 * FP_SLOTS;
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_s;
+    __shared__ volatile FpEnd end_s;
     __shared__ uint32_t most[GATED ? 2 : 1][2][FT_ROWS];
     __shared__ __align__(8) uint64_t met[4];            // the two warps of a quarter of the lanes tell each other their maxima
     const int warp = ft_warp(), lane = threadIdx.x & 31;
@@ -150,6 +183,8 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const int pair = blockIdx.x >> 1, n_pairs = gridDim.x >> 1, n_items = p.tiles_m * p.tiles_n;
     if (threadIdx.x == 0) {
         abort_s = 0;
+        end_s.tiles = tiles_addr;
+        end_s.asked = end_s.issued = end_s.other_abort = 0;
         for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
         for (int b = 0; b < FP_SLOTS; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, 16); }
         for (int q = 0; q < 4; ++q) mbar_init(gt_smem(&met[q]), 2);
@@ -214,7 +249,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 ready = __all_sync(0xffffffffu, ft_ready(empty0 + 8 * s, ph ^ 1));
             }
         }
-        if (failed && rank == 0) ft_drain(full0, STAGES, asked, p.wait_limit);
+        if (lane == 0) end_s.asked = asked;
     } else if (warp == 1) {
         if (rank == 0) {
             pdl_wait();         // (the first tokens come after it: the wait for them starts there)
@@ -242,6 +277,7 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                     ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));       // (the next k-block has landed)
                 }
             }
+            if (lane == 0) end_s.issued = (int)turn;
         }
     } else {
         const int wq = warp & 3, part = (warp - 2) >> 2;
@@ -334,10 +370,19 @@ gemm_fp8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             }
         }
     }
-    // neither CTA leaves, nor is the pair's tensor memory given back, while the other may still use this one's
+    // Neither CTA leaves, nor is the pair's tensor memory given back, while the other may still use this one's.  Each tells the other whether
+    // it gave up and how many k-blocks it asked for: a barrier of the leader's counts both CTAs' loads.
     tc_fence_before();
     __syncthreads();
+    if (threadIdx.x == 0) {
+        ft_tell(cluster_map(gt_smem(const_cast<const int*>(&end_s.other_asked)), cluster_ctarank() ^ 1), end_s.asked);
+        ft_tell(cluster_map(gt_smem(const_cast<const int*>(&end_s.other_abort)), cluster_ctarank() ^ 1), abort_s);
+    }
     cluster_sync_all();
+    if (abort_s | end_s.other_abort) {
+        if (threadIdx.x < 32) fp_settle<COLS>(end_s, p.stages, &map_x, &map_w);
+        cluster_sync_all();
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512));
@@ -372,6 +417,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     const uint32_t tfull0 = empty0 + 8 * STAGES, tempty0 = tfull0 + 8 * S::SLOTS;
     __shared__ uint32_t tmem_base_s;
     __shared__ volatile int abort_s;
+    __shared__ int asked_s, issued_s;           // k-blocks whose loads and whose products are issued
     const int warp = ft_warp(), lane = threadIdx.x & 31;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, ta = tile % p.tiles_m, tb = tile / p.tiles_m;
     const int kb0 = split * p.kb_per_split, kb1 = min(kb0 + p.kb_per_split, p.n_kb);
@@ -436,7 +482,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             if (++s == STAGES) { s = 0; ph ^= 1; }
             ready = __all_sync(0xffffffffu, ft_ready(empty0 + 8 * s, ph ^ 1));
         }
-        if (failed || abort_s) ft_drain(full0, STAGES, asked, p.wait_limit);
+        if (lane == 0) asked_s = asked;
     } else if (warp == 1) {
         pdl_wait();
         const uint32_t idesc = ft_idesc(BN, FT_ROWS);
@@ -444,7 +490,8 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         uint32_t ph = 0;
         int s = 0;
         bool ready = false;
-        for (int turn = 0; turn < count; ++turn) {
+        int turn = 0;
+        for (; turn < count; ++turn) {
             const uint32_t buf = (uint32_t)turn % S::SLOTS, use = (uint32_t)turn / S::SLOTS;
             if ((!ready && ft_warp_failed(full0 + 8 * s, ph, &abort_s, p, 3)) ||
                 (use && ft_warp_failed(tempty0 + 8 * buf, (use & 1) ^ 1, &abort_s, p, 2)))
@@ -462,6 +509,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             if (++s == STAGES) { s = 0; ph ^= 1; }
             ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));
         }
+        if (lane == 0) issued_s = turn;
     } else {
         const int wq = warp & 3, part = (warp - 2) >> 2;
         pdl_wait();
@@ -510,6 +558,10 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
+        if (abort_s) {
+            ft_drain(full0, STAGES, asked_s);
+            ft_drain(empty0, STAGES, issued_s);
+        }
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }
