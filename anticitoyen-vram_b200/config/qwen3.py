@@ -11,6 +11,7 @@ holds a size.
 
 from __future__ import annotations
 
+import re
 from dataclasses import dataclass, asdict
 from typing import Any, Mapping
 
@@ -71,16 +72,17 @@ class Qwen3Config:
             hidden_act=str(act),
             eos_token_id=take_id_list(cfg, "eos_token_id"),
             bos_token_id=bos if isinstance(bos, int) and not isinstance(bos, bool) else None,
-            weights_fp8=cls._weights_fp8(cfg),
+            weights_fp8=cls._weights_fp8(cfg, take_int(cfg, "num_hidden_layers", 32)),
         )
         self._check_unsupported(cfg)
         self.validate()
         return self
 
     @staticmethod
-    def _weights_fp8(cfg: Mapping[str, Any]) -> bool:
+    def _weights_fp8(cfg: Mapping[str, Any], layers: int) -> bool:
         """Whether the configuration asks for 8-bit weights; what is built of them is the form with block scales and activations
-        quantised as they come.  (Other methods are no business of this key's reader: their files hold other tensors.)"""
+        quantised as they come, in all of a layer's seven matrices: a list of modules that stay in more bits may name others only.
+        (Other methods are no business of this key's reader: their files hold other tensors.)"""
         quant = cfg.get("quantization_config")
         if not isinstance(quant, Mapping) or quant.get("quant_method") != "fp8":
             return False
@@ -88,6 +90,18 @@ class Qwen3Config:
             got = quant.get(key, default)
             if (list(got) if isinstance(got, (list, tuple)) else got) != want:
                 raise ConfigError(f"config key 'quantization_config': '{key}' is {got!r}; of 8-bit weights {want!r} is built")
+        matrices = [f"model.layers.{i}.{part}_proj.weight" for i in range(layers)
+                    for part in ("self_attn.q", "self_attn.k", "self_attn.v", "self_attn.o", "mlp.gate", "mlp.up", "mlp.down")]
+        for key in ("modules_to_not_convert", "ignored_layers"):
+            kept = quant.get(key) or []
+            if not isinstance(kept, (list, tuple)) or not all(isinstance(k, str) and re.fullmatch(r"[\w.]+", k) for k in kept):
+                raise ConfigError(f"config key 'quantization_config': '{key}' is {kept!r}; a list of modules' names is read")
+            # (readers of this list compare whole names, beginnings, ends or parts: what any of them would keep is refused)
+            for name in kept:
+                hit = next((m for m in matrices if name in m or m.removesuffix(".weight") in name), None)
+                if hit is not None:
+                    raise ConfigError(f"config key 'quantization_config': '{key}' names '{name}', which keeps {hit} in more bits; "
+                                      "8-bit weights are built for all of a layer's matrices")
         return True
 
     @staticmethod
