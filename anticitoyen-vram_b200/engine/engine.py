@@ -100,14 +100,18 @@ class Engine:
         ``fuse_decode_layers``: steps of up to 16 decoding requests run each layer as one persistent kernel instead
         of seven launches (slower on a B200 at the sizes measured; kept as a choice).
         ``weights``: None, as the model's configuration says; "fp8" (Qwen3): the layers' matrices in e4m3 with a scale for
-        each block of 128 x 128, quantised as they are loaded where the folder holds them in more bits."""
+        each block of 128 x 128, quantised as they are loaded where the folder holds them in more bits (not with a model
+        that is already built)."""
         from ..config import load_config
         from ..models import build_from_folder, build_random, with_weights
 
         run_dtype = _DTYPES[dtype]
+        built = hasattr(model, "plan") and hasattr(model, "forward")     # a model already built and loaded
+        if built and weights is not None:
+            raise ValueError(f"weights '{weights}': the model is already built, and its weights stay what they are")
         if not torch.cuda.is_available():
             raise RuntimeError("acvram_b200 needs a CUDA device: its kernels have no CPU path")
-        if hasattr(model, "plan") and hasattr(model, "forward"):     # a model already built and loaded
+        if built:
             self.model, self.config = model, None
         elif random_weights:
             config = load_config(model) if isinstance(model, (str, bytes)) or hasattr(model, "__fspath__") else model

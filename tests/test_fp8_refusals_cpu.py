@@ -43,3 +43,17 @@ def test_a_list_that_cannot_be_read_is_refused(names):
 def test_the_list_of_another_method_is_not_read():
     from acvram_b200.config import Qwen3Config
     assert not Qwen3Config.from_dict(fp8_config(quant_method="other", modules_to_not_convert=["q_proj"])).weights_fp8
+
+
+def test_weights_in_8_bits_are_not_asked_of_a_model_already_built():
+    """Its weights would stay in more bits."""
+    from acvram_b200 import Engine
+
+    class Built:
+        plan = None
+
+        def forward(self):
+            raise AssertionError
+
+    with pytest.raises(ValueError, match="already built"):
+        Engine(Built(), weights="fp8")
