@@ -2428,23 +2428,28 @@ def _one_device(name: str, *tensors) -> None:
         raise KernelError(f"{name}: the tensors lie on different devices")
 
 
-def _dense(name: str, what: str, t: torch.Tensor, shape: tuple, dtypes: tuple) -> None:
-    """Raises unless t is a matrix of that shape and one of those types, its rows dense."""
+def _dense(name: str, what: str, t: torch.Tensor, shape: tuple, dtypes: tuple, written: bool = False) -> None:
+    """Raises unless t is a matrix of that shape and one of those types, its rows dense, and apart where they are ``written``."""
     if t.dtype not in dtypes or tuple(t.shape) != shape or (t.stride(1) != 1 and shape[1] > 1):
         raise KernelError(f"{name}: {what} must be {' or '.join(str(d).removeprefix('torch.') for d in dtypes)} {list(shape)} with dense rows, "
                           f"got {str(t.dtype).removeprefix('torch.')} {list(t.shape)} strides {t.stride()}")
+    if written and shape[0] > 1 and t.stride(0) < shape[1]:
+        raise KernelError(f"{name}: the rows of {what} overlap, and they are written: {list(t.shape)} strides {t.stride()}")
 
 
-def _fp8_pair(name: str, what: str, values: torch.Tensor, scales: torch.Tensor, rows: int, columns: int, block_rows: int) -> None:
+def _fp8_pair(name: str, what: str, values: torch.Tensor, scales: torch.Tensor, rows: int, columns: int, block_rows: int,
+              written: bool = False) -> None:
     """Raises unless (values, scales) are a quantised matrix of that size with dense rows."""
-    _dense(name, what, values, (rows, columns), (FP8,))
-    _dense(name, "the scales of " + what, scales, (rows if block_rows == 1 else (rows + 127) // 128, (columns + 127) // 128), (torch.float32,))
+    _dense(name, what, values, (rows, columns), (FP8,), written)
+    _dense(name, "the scales of " + what, scales, (rows if block_rows == 1 else (rows + 127) // 128, (columns + 127) // 128),
+           (torch.float32,), written)
 
 
 def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, block_rows: int = 1) -> tuple[torch.Tensor, torch.Tensor]:
     """(values, scales) of x [R, C] (float32 or bfloat16, dense rows at any stride), in groups of 128 of a row (``block_rows`` 1) or
-    in blocks of 128 x 128 (``block_rows`` 128): s = max(largest magnitude / 448, 2^-126), value = e4m3(x * (1 / s)), each step
-    rounded once.  A group with a NaN becomes NaN as a whole; one with an infinity gets an infinite scale."""
+    in blocks of 128 x 128 (``block_rows`` 128), the result's rows apart: s = max(largest magnitude / 448, 2^-126),
+    value = e4m3(x * (1 / s)), each step rounded once.  A group with a NaN becomes NaN as a whole; one with an infinity gets an
+    infinite scale."""
     shape, dtype, device = x.shape, x.dtype, x.get_device()
     if len(shape) != 2 or block_rows not in (1, 128):
         raise KernelError("quantize_fp8: a matrix, and block_rows 1 or 128, are wanted")
@@ -2452,9 +2457,10 @@ def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, bl
     xs, vs, ss = x.stride(), values.stride(), scales.stride()
     if not (dtype in _DT and values.dtype is FP8 and scales.dtype is torch.float32 and values.shape == shape
             and scales.shape == (R if block_rows == 1 else (R + 127) // 128, (C + 127) // 128) and xs[1] == 1 and vs[1] == 1 and ss[1] == 1
+            and (R < 2 or vs[0] >= C and ss[0] >= scales.shape[1])
             and device >= 0 and values.get_device() == device and scales.get_device() == device):
         _dense("quantize_fp8", "x", x, (R, C), (torch.float32, torch.bfloat16))
-        _fp8_pair("quantize_fp8", "the result", values, scales, R, C, block_rows)
+        _fp8_pair("quantize_fp8", "the result", values, scales, R, C, block_rows, True)
         _one_device("quantize_fp8", x, values, scales)
     if R and C:
         _launch_record(device, "quantize_fp8", _QUANTIZE_ARGS, 3, x.data_ptr(), values.data_ptr(), scales.data_ptr(), xs[0], vs[0], ss[0],
@@ -2465,8 +2471,9 @@ def quantize_fp8(x: torch.Tensor, values: torch.Tensor, scales: torch.Tensor, bl
 def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scales: torch.Tensor, out: torch.Tensor,
                static_weights: bool = False, plan: tuple | None = None) -> torch.Tensor:
     """out[T, N] = x @ w^T of quantised matrices: x [T, K] with a scale for each group of 128 of a row, w [N, K] with a scale for each
-    block of 128 x 128; out float32 or bfloat16, dense rows at any stride.  A group's sum is multiplied by its two scales' float
-    product and joins a float sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``) and do not overlap.
+    block of 128 x 128; out float32 or bfloat16, dense rows at any stride that keeps them apart.  A group's sum is multiplied by its
+    two scales' float product (scales whose product is beyond a float give no numbers, even where the sum is zero) and joins a float
+    sum, which is rounded once.  The rows of x and w start on 16 bytes (``fp8_rows``) and do not overlap.
 
     ``static_weights``: w and its scales were written long before this call (a model's weights), so the kernel may read them while
     the kernels before it in the stream are still running.  ``plan``: (kind, columns of a tile, splits of K) as csrc/gemm_fp8_tc.cu
@@ -2478,11 +2485,11 @@ def linear_fp8(x: torch.Tensor, x_scales: torch.Tensor, w: torch.Tensor, w_scale
     device = x.get_device()
     if not (Kw == K and x.dtype is FP8 and w.dtype is FP8 and x_scales.dtype is torch.float32 and w_scales.dtype is torch.float32
             and out.dtype in _DT and x_scales.shape == (T, G) and w_scales.shape == ((N + 127) // 128, G) and out.shape == (T, N)
-            and xs[1] == 1 and xss[1] == 1 and ws[1] == 1 and wss[1] == 1 and outs[1] == 1 and device >= 0
+            and xs[1] == 1 and xss[1] == 1 and ws[1] == 1 and wss[1] == 1 and outs[1] == 1 and (T < 2 or outs[0] >= N) and device >= 0
             and x_scales.get_device() == device and w.get_device() == device and w_scales.get_device() == device and out.get_device() == device):
         _fp8_pair("linear_fp8", "x", x, x_scales, T, K, 1)
         _fp8_pair("linear_fp8", "w", w, w_scales, N, K, 128)
-        _dense("linear_fp8", "out", out, (T, N), (torch.float32, torch.bfloat16))
+        _dense("linear_fp8", "out", out, (T, N), (torch.float32, torch.bfloat16), True)
         _one_device("linear_fp8", x, x_scales, w, w_scales, out)
     if not T or not N:
         return out
@@ -2510,13 +2517,14 @@ def linear_fp8_swiglu(x: torch.Tensor, x_scales: torch.Tensor, gate: torch.Tenso
             and gate_scales.dtype is torch.float32 and up_scales.dtype is torch.float32 and out_scales.dtype is torch.float32
             and up.shape == (I, K) and x_scales.shape == (T, G) and gate_scales.shape == (B, G) and up_scales.shape == (B, G)
             and out.shape == (T, I) and out_scales.shape == (T, B) and xs[1] == 1 and xss[1] == 1 and gs[1] == 1 and gss[1] == 1
-            and us[1] == 1 and uss[1] == 1 and outs[1] == 1 and outss[1] == 1 and device >= 0 and x_scales.get_device() == device
+            and us[1] == 1 and uss[1] == 1 and outs[1] == 1 and outss[1] == 1 and (T < 2 or outs[0] >= I and outss[0] >= B)
+            and device >= 0 and x_scales.get_device() == device
             and gate.get_device() == device and gate_scales.get_device() == device and up.get_device() == device
             and up_scales.get_device() == device and out.get_device() == device and out_scales.get_device() == device):
         _fp8_pair("linear_fp8_swiglu", "x", x, x_scales, T, K, 1)
         _fp8_pair("linear_fp8_swiglu", "gate", gate, gate_scales, I, K, 128)
         _fp8_pair("linear_fp8_swiglu", "up", up, up_scales, I, K, 128)
-        _fp8_pair("linear_fp8_swiglu", "the result", out, out_scales, T, I, 1)
+        _fp8_pair("linear_fp8_swiglu", "the result", out, out_scales, T, I, 1, True)
         _one_device("linear_fp8_swiglu", x, x_scales, gate, gate_scales, up, up_scales, out, out_scales)
     if not T or not I:
         return out, out_scales
@@ -2541,14 +2549,15 @@ def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tens
 
     x and delta float32 or bfloat16; ``gate`` float32 [H], or [T, H] float32 or bfloat16; weights float32 [H].  out float32 or
     bfloat16, rounded once, or float8_e4m3fn with ``out_scales``: quantised in groups of 128 as ``quantize_fp8`` does.  Matrices
-    have dense rows at any stride; H up to 16384.  Sums and both statistics are 32-bit.  ``static_weights``: the weights and a gate of [H]
-    were written long before this call and may be read while the kernels before it are still running."""
+    have dense rows at any stride, those that are written apart; H up to 16384.  Sums and both statistics are 32-bit.
+    ``static_weights``: the weights and a gate of [H] were written long before this call and may be read while the kernels before it
+    are still running."""
     shape, device = x.shape, x.get_device()
     T, H = shape
     floats = (torch.float32, torch.bfloat16)
     name = "add_gated_norms"
     xs = x.stride()
-    ok = x.dtype in _DT and xs[1] == 1 and device >= 0
+    ok = x.dtype in _DT and xs[1] == 1 and (T < 2 or xs[0] >= H) and device >= 0
     d_at = d_type = d_ld = g_at = g_type = g_ld = gc_at = w1_at = w2_at = out_at = out_ld = s_at = s_ld = 0
     kind = 3
     if delta is not None:
@@ -2574,17 +2583,19 @@ def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tens
             raise KernelError("add_gated_norms: a result wants a weight")
         kind = _NORM_OUT.get(out.dtype, 3)
         outs = out.stride()
-        ok = ok and kind < 3 and out.shape == shape and outs[1] == 1 and out.get_device() == device and (kind == 2) == (out_scales is not None) \
+        ok = ok and kind < 3 and out.shape == shape and outs[1] == 1 and (T < 2 or outs[0] >= H) and out.get_device() == device \
+            and (kind == 2) == (out_scales is not None) \
             and weight.dtype is torch.float32 and weight.shape == (H,) and weight.stride(0) == 1 and weight.get_device() == device
         w2_at, out_at, out_ld = weight.data_ptr(), out.data_ptr(), outs[0]
         if out_scales is not None:
             ss = out_scales.stride()
-            ok = ok and out_scales.dtype is torch.float32 and out_scales.shape == (T, (H + 127) // 128) and ss[1] == 1 and out_scales.get_device() == device
+            ok = ok and out_scales.dtype is torch.float32 and out_scales.shape == (T, (H + 127) // 128) and ss[1] == 1 \
+                and (T < 2 or ss[0] >= out_scales.shape[1]) and out_scales.get_device() == device
             s_at, s_ld = out_scales.data_ptr(), ss[0]
     elif out_scales is not None:
         raise KernelError("add_gated_norms: scales without a result")
     if not ok:
-        _dense(name, "x", x, (T, H), floats)
+        _dense(name, "x", x, (T, H), floats, True)
         if delta is not None:
             _dense(name, "delta", delta, (T, H), floats)
         if g_at:
@@ -2595,9 +2606,9 @@ def add_gated_norms(x: torch.Tensor, delta: torch.Tensor | None, out: torch.Tens
         if out is not None:
             if (out.dtype == FP8) != (out_scales is not None):
                 raise KernelError(f"{name}: out_scales go with a result of float8_e4m3fn, and only with one")
-            _dense(name, "out", out, (T, H), tuple(_NORM_OUT))
+            _dense(name, "out", out, (T, H), tuple(_NORM_OUT), True)
             if out_scales is not None:
-                _fp8_pair(name, "out", out, out_scales, T, H, 1)
+                _fp8_pair(name, "out", out, out_scales, T, H, 1, True)
         _one_device(name, x, delta, gate, post_weight, weight if out is not None else None, out, out_scales)
     if T and H:
         _launch_record(device, name, _NORMS_ARGS, 8, x.data_ptr(), d_at, g_at, gc_at, w1_at, w2_at, out_at, s_at, xs[0], d_ld, g_ld, out_ld,

@@ -57,3 +57,53 @@ def test_weights_in_8_bits_are_not_asked_of_a_model_already_built():
 
     with pytest.raises(ValueError, match="already built"):
         Engine(Built(), weights="fp8")
+
+
+# ----------------------------------------------------------------------------- results whose rows overlap
+def overlapping(t, by=1):
+    """A view of t's memory with rows `by` elements less apart than they are long."""
+    return t.as_strided(t.shape, (t.shape[1] - by, 1))
+
+
+def test_results_whose_rows_overlap_are_refused():
+    """Two rows' kernels would write the same elements, and the stream's be read by one when the other has written it."""
+    import torch
+
+    from acvram_b200.kernels import ops
+    x, w = torch.zeros((4, 256)), torch.zeros(256)
+    q, s = ops.fp8_rows(4, 256, "cpu")
+    wq, ws = ops.fp8_rows(256, 256, "cpu")[0], torch.empty((2, 2))
+    out = torch.empty((4, 256))
+    one = lambda t: t[:1].expand(t.shape)
+    calls = [(ops.quantize_fp8, (x, one(q), s), {}), (ops.quantize_fp8, (x, q, overlapping(s)), {}),
+             (ops.quantize_fp8, (torch.zeros((256, 256)), wq, one(ws), 128), {}),
+             (ops.linear_fp8, (q, s, wq, ws, one(out)), {}), (ops.linear_fp8, (q, s, wq, ws, overlapping(out)), {}),
+             (ops.linear_fp8_swiglu, (q, s, wq, ws, wq, ws, overlapping(q), s), {}),
+             (ops.linear_fp8_swiglu, (q, s, wq, ws, wq, ws, q, one(s)), {}),
+             (ops.add_gated_norms, (one(x), x, q, s), {"weight": w}), (ops.add_gated_norms, (overlapping(x, 200), None, out), {"weight": w}),
+             (ops.add_gated_norms, (x, x, overlapping(out), None), {"weight": w}), (ops.add_gated_norms, (x, x, one(q), s), {"weight": w}),
+             (ops.add_gated_norms, (x, x, q, one(s)), {"weight": w})]
+    for call, args, kw in calls:
+        with pytest.raises(ops.KernelError, match="overlap"):
+            call(*args, **kw)
+
+
+def test_a_single_row_and_operands_that_are_only_read_may_have_any_stride():
+    """These get as far as the question of the device."""
+    import torch
+
+    from acvram_b200.kernels import ops
+    x, w = torch.zeros((4, 256)), torch.zeros(256)
+    q, s = ops.fp8_rows(4, 256, "cpu")
+    wq, ws = ops.fp8_rows(256, 256, "cpu")[0], torch.empty((2, 2))
+    out = torch.empty((4, 256))
+    one = lambda t: t[:1].expand(t.shape)
+    narrow = lambda t: t.as_strided((1, t.shape[1]), (0, 1))
+    calls = [(ops.quantize_fp8, (one(x), q, s), {}), (ops.quantize_fp8, (x[:1], narrow(q), narrow(s)), {}),
+             (ops.linear_fp8, (q, one(s), wq, one(ws), out), {}), (ops.linear_fp8, (q[:1], s[:1], wq, ws, narrow(out)), {}),
+             (ops.linear_fp8_swiglu, (q[:1], s[:1], wq, ws, wq, ws, narrow(q), narrow(s)), {}),
+             (ops.add_gated_norms, (x, one(x), q, s), {"weight": w, "gate": one(x)}),
+             (ops.add_gated_norms, (narrow(x), x[:1], narrow(q), narrow(s)), {"weight": w})]
+    for call, args, kw in calls:
+        with pytest.raises(ops.KernelError, match="CPU tensor"):
+            call(*args, **kw)
