@@ -63,6 +63,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
     // (only now may the next kernel's CTAs come: one that took tensor memory before this CTA had its own could wait for this grid)
     pdl_launch_dependents();
 
+    bool failed = false;            // this warp gave up a wait
     if (warp == 0) {
         auto load_w = [&](int s, int kb) {
             tma_load_2d(tiles_addr + s * S::STAGE, &map_w, full0 + 8 * s, kb * FT_ROWS, tb * FT_ROWS + half * 64);
@@ -79,7 +80,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         pdl_wait();
         int s = 0, asked = 0;
         uint32_t ph = 0;
-        bool failed = false, ready = false;
+        bool ready = false;
         for (; asked < count; ++asked) {
             const bool half_done = asked < early;
             const int kb = kb0 + block_of(asked);
@@ -124,6 +125,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             if (++s == STAGES) { s = 0; ph ^= 1; }
             ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));
         }
+        failed = i < count;
         if (lane == 0) issued_s = i;
     } else {
         const int wq = warp & 3, et = threadIdx.x - 64;
@@ -163,7 +165,8 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         uint32_t turn = 0;
         for (int i = 0; i < count; ++i, ++turn) {
             const uint32_t slot = turn % S::SLOTS, use = turn / S::SLOTS;
-            if (ft_warp_failed(tfull0 + 8 * slot, use & 1, &abort_s, p)) break;
+            failed = ft_warp_failed(tfull0 + 8 * slot, use & 1, &abort_s, p);
+            if (failed) break;
             tc_fence_after();
             const ulonglong2* sc = reinterpret_cast<const ulonglong2*>(own_scales + block_of(i) * (HALVES * BT));
 #pragma unroll
@@ -193,11 +196,11 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
             }
         }
     }
-    // (tensor memory goes back before the cluster's CTAs wait for one another, see gemm_fp8_tc.cu)
+    // (tensor memory goes back before the cluster's CTAs wait for one another, and the barrier says whether a warp gave up, see gemm_fp8_tc.cu)
     tc_fence_before();
-    __syncthreads();
+    const bool gave_up = __syncthreads_or(failed);
     if (warp == 1) {
-        if (abort_s) {
+        if (gave_up) {
             ft_drain(full0, STAGES, asked_s);
             ft_drain(empty0, STAGES, issued_s);
         }
@@ -205,7 +208,7 @@ gemm_fp8_narrow_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_c
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }
     if (size > 1) cluster_sync_all();
-    if (!abort_s)
+    if (!gave_up)
         ft_emit<FT_ROWS, GATED, HALVES, 1, 8 / HALVES>(p, tiles_addr, S::LD, rank + size * warp, size * (FN_THREADS / 32), min(BT, p.M - t0), t0, tb);
     // (the peers may still read this CTA's sums)
     if (size > 1) cluster_sync_all();

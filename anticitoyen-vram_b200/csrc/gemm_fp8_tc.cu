@@ -442,6 +442,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     // all read the same tokens' bytes at the same time (a tile's order is its own, whatever the others do).
     const int count = kb1 - kb0, turned = (int)(ft_spread(tb) % (unsigned)((count + 3) / 4)) * 4, wrap = count - turned;
     auto block_of = [&](int i) { return i < wrap ? i + turned : i - wrap; };
+    bool failed = false;            // this warp gave up a wait
     if (warp == 0) {
         auto load_w = [&](int s, int kb) {
             const uint32_t dst = tiles_addr + s * S::STAGE + FT_TILE;
@@ -463,7 +464,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         pdl_wait();
         int s = 0, asked = 0;
         uint32_t ph = 0;
-        bool failed = false, ready = false;
+        bool ready = false;
         for (; asked < count; ++asked) {
             const bool half_done = asked < early;
             const int kb = kb0 + block_of(asked);
@@ -509,6 +510,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
             if (++s == STAGES) { s = 0; ph ^= 1; }
             ready = __all_sync(0xffffffffu, ft_ready(full0 + 8 * s, ph));
         }
+        failed = turn < count;
         if (lane == 0) issued_s = turn;
     } else {
         const int wq = warp & 3, part = (warp - 2) >> 2;
@@ -532,7 +534,8 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
                 if (GATED) next_w2 = sw2[block_of(turn + 1)];
             }
             const uint32_t buf = (uint32_t)turn % S::SLOTS, use = (uint32_t)turn / S::SLOTS;
-            if (ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p)) break;
+            failed = ft_warp_failed(tfull0 + 8 * buf, use & 1, &abort_s, p);
+            if (failed) break;
             tc_fence_after();
             const uint32_t t = taddr + buf * BN;
             if (GATED) ft_add_tile<S::COLS / 16>(sums, t + part * 64, t + FT_ROWS + part * 64, s1, s2);
@@ -555,10 +558,11 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
     }
     // Tensor memory goes back before the cluster's CTAs wait for one another: a CTA that held some while it waited for a peer, which waits for
     // some that another kernel's CTA holds in the same way, would wait for good.
+    // (Whether a warp gave up comes with the barrier: a look at the flag behind it took 0.05 us of every kernel's end.)
     tc_fence_before();
-    __syncthreads();
+    const bool gave_up = __syncthreads_or(failed);
     if (warp == 1) {
-        if (abort_s) {
+        if (gave_up) {
             ft_drain(full0, STAGES, asked_s);
             ft_drain(empty0, STAGES, issued_s);
         }
@@ -566,7 +570,7 @@ gemm_fp8_tile_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_con
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(S::TMEM));
     }
     if (p.splits > 1) cluster_sync_all();
-    if (!abort_s) {
+    if (!gave_up) {
         const int first = split + p.splits * warp, step = p.splits * (S::THREADS / 32), rows = min(FT_ROWS, p.M - row_here);
         if (p.splits == 1) ft_emit<BN, GATED, 1, 4, 1>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
         else if (p.splits <= 4 && rows > 2 * step) ft_emit<BN, GATED, 1, 4, 4>(p, tiles_addr, S::LD, first, step, rows, row_here, tb);
