@@ -191,7 +191,7 @@ class PreNormBlock:
 
     def _normed(self, norm, x, delta, part, kw: dict, scale: dict):
         """The sum and its norm, in 8 bits where the part behind it reads that."""
-        if part.takes_fp8 and getattr(norm, "groups", 0) == 1 and x.shape[1] <= ops.GATED_NORMS_WIDTH:
+        if getattr(part, "takes_fp8", False) and getattr(norm, "groups", 0) == 1 and x.shape[1] <= ops.GATED_NORMS_WIDTH:
             return norm.forward_fp8(x, delta, self.run_dtype, **scale)
         return norm.forward(x, delta, **kw, **scale)
 
