@@ -220,6 +220,8 @@ class ParallelBlock:
             for part in (self.mixer, self.feed_forward):
                 if not hasattr(part, "inner_size") or not hasattr(part, "inner"):
                     raise ValueError(f"a '{part.kind}' part cannot stand beside another one (it offers no inner columns)")
+                if getattr(part, "takes_fp8", False):
+                    raise ValueError(f"a '{part.kind}' part with 8-bit weights cannot stand beside another one (its last product has scales of its own)")
         self.run_dtype = None
         self.out = None
 

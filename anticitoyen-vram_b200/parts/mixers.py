@@ -534,6 +534,8 @@ class ParallelMixers(Mixer):
         for side in (self.left, self.right):
             if not all(hasattr(side, a) for a in ("in_size", "inner_size", "mix")):
                 raise ValueError(f"a '{side.kind}' mixer cannot stand beside another one (it offers no mix())")
+            if getattr(side, "takes_fp8", False):
+                raise ValueError(f"a '{side.kind}' mixer with 8-bit weights cannot stand beside another one (its products have scales of their own)")
 
     def metadata_providers(self) -> dict:
         return {**self.right.metadata_providers(), **self.left.metadata_providers()}
