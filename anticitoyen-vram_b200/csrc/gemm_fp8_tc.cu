@@ -6,7 +6,7 @@
 // tensor memory for one k-block.  It cannot stay there: its scales differ from k-block to k-block.  Tensor memory holds several such
 // partial tiles; while the tensor core fills one, the epilogue warps fetch another and add it, times its scales, to the float
 // sums that they hold in registers (a fused multiply-add for each output and k-block, two at a time as fma.rn.f32x2).  Tokens are
-// the rows (a lane holds one, so sx is a number of the thread's), features the columns, 64 or 128 of them to a thread.
+// the rows (a lane holds one, so sx is a number of the thread's), features the columns, 64 to 128 of them to a thread.
 //
 // Two forms.  Pairs of CTAs on tiles of 256 x 256 or somewhat less (cta_group::2), persistent, for many tokens: a CTA loads 128 rows of each
 // operand for a k-block, 32 KB for 512 cycles of tensor core.  And single CTAs on tiles of 128 x BN, one each, for fewer: K may be split over
@@ -19,8 +19,8 @@
 // sixteen warps 310).
 //
 // Warps: 0 loads, 1 issues the products, from 2 on they are the epilogue, each a quarter of the lanes.  Every wait on an mbarrier is
-// bounded; when one runs out the kernel records where in `status`, all roles leave their loops, the loads in flight are waited for
-// (with a limit), tensor memory is freed and the kernel returns.
+// bounded; when one runs out the kernel records where in `status`, all roles leave their loops, the loads and products under way are
+// waited for (with a limit, ft_drain), tensor memory is freed and the kernel returns.
 #include "fp8_tc.cuh"
 
 // sums[0 .. 8 PIECES) += scales * 16 PIECES columns of this lane's row, the first half of them from `first`, the others from `second`;
@@ -656,7 +656,7 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
     return acv_launch_status();
 }
 
-// How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs on tiles of 256 x bn, 4 weight
+// (Microseconds of calls in bursts, before the board's power cap is felt.)  How a product is made: kind 1 the streaming kernel (gemm_fp8_rows.cu), 2 tiles of 128 x bn with K over `splits` CTAs, 3 pairs on tiles of 256 x bn, 4 weight
 // rows on the tensor core's rows, bn tokens to a tile, K over `splits` CTAs (gemm_fp8_narrow.cu).
 //
 // Up to 16 tokens whose weights are one round of blocks of 32 rows stream (microseconds, streaming and the best of kind 4: 8 tokens
@@ -665,13 +665,14 @@ static int ft_launch_tile(const CUtensorMap& mx, const CUtensorMap& mw, const CU
 // 4096 x 12288 15.9 and 14.0, 5120 x 17408 20.8 and 20.8.
 //   Splits of K are what fits the SMs at once in clusters, two CTAs of kind 4 to an SM (three of the gated form, whose cluster holds two
 // halves of a group), one of kind 2, and at least four k-blocks to each: 16 tokens 6144 x 4096 in 2, 4, 6 splits 7.9, 6.1, 9.8; 4096 x 1024
-// in 1, 2, 4: 4.3, 3.8, 4.2; 12288 units, K 4096, in 1, 2, 3: 21.0, 19.2, 24.8; kind 2, 65 tokens 4096 x 12288 in 2, 3, 4, 6: 19.5, 15.9,
+// in 1, 2, 4: 4.3, 3.8, 4.2; 12288 units, K 4096, in 1, 2, 3: 21.0, 19.2, 24.8 (the gated form stays with two: where few units leave SMs idle
+// four would be faster, 32 tokens, 1361 units of 11216 in 2 and 4: 18, 12; 3000 units of 4096: 10.3, 9.5); kind 2, 65 tokens 4096 x 12288 in 2, 3, 4, 6: 19.5, 15.9,
 // 14.0, 23.3.  Kind 4 holds the scales of its k-blocks in shared memory beside its stages: 160 KB of them at most, about 80 thousand k to a
 // split of 32 tokens' gated form, and longer rows are kind 2's (one that holds none).
 //   Pairs of CTAs and tiles of 128 rows both come in rounds over the SMs.  A round of pairs takes 1.5 of a round of tiles of 128 x 128
 // (1024 tokens 5120 x 17408 in 2 and 3: 143 us and 136; 6144 x 4096, 512 tokens in 1 and 2: 28, 32; 2048 in 3 and 6: 63, 82), 0.83 of
 // one of gated tiles of 128 x 256 (12288 units of 4096, 256 tokens in 2 and 2: 43.8, 50.1; 384 in 3 and 2: 69, 54), and K over several CTAs brings a
-// round of those down with it (100 tokens of 8704 units of 5120, pairs and 2 splits: 31, 26; 39 of 1361 units of 11216, pairs and 8: 49, 16).  Pairs take tiles of
+// round of those down with it (100 tokens of 8704 units of 5120, pairs and 2 splits: 31, 26; 39 of 1361 units of 11216, pairs and 8: 49, 13).  Pairs take tiles of
 // 256 columns, or of 224 or 192 where those come in few enough rounds: such a round takes 0.94 and 0.87 (with 256, 224 and 192 columns, 1024
 // tokens 7168 x 5120 in 2, 2, 3 rounds 49.7, 46.1, 57.4; 5120 x 17408 in 2, 2, 2: 143, 135, 122; 4096 tokens 4096 x 12288 in 4, 5, 5: 202, 257, 234).
 struct Fp8Plan { int kind, bn, splits; };
